@@ -455,6 +455,158 @@ uint64_t vvli_cuda_moe_workspace_bytes(uint64_t tokens, uint64_t hidden, uint64_
                                        uint64_t top_k);
 int vvli_cuda_moe_ffn(int device, const vvli_moe_args* args, void* stream);
 
+/* ---------------------------------------------------------------- paged serving step
+ * Four operators over a 16-bit paged KV cache that the caller owns, for steps
+ * with several new tokens per request (a decode token, a prompt chunk, or
+ * drafted tokens): page planning, q / k norm + rotation + cache write,
+ * attention, draft verification.  No counterpart in the reference, whose
+ * KVCache (src/llm.zig:539-606) is one contiguous fp32 sequence; the layout is
+ * this runtime's own: a cache is [pages][kv heads][page_size][head_dim] with
+ * pages page_stride elements apart, page_size 16, 32, 64 or 128, and row b of
+ * a block table lists request b's pages in position order.
+ *
+ * All of them need no context and allocate nothing; pointers are device
+ * memory of `device`.  The work is queued on `stream` (a cudaStream_t; NULL =
+ * the legacy default stream), may be captured into a graph (after one call of
+ * the operator on that device outside a capture), and the caller's current
+ * device is restored.  Sizes, types, alignments and pointers outside the
+ * limits below return VVLI_ERR_INVALID_ARGUMENT before anything is queued,
+ * with the reason in vvli_cuda_last_error(); values in device memory are
+ * bounds-checked by the kernels instead, as described with each operator. */
+enum vvli_dtype {
+  VVLI_BF16 = 0,
+  VVLI_FP16 = 1
+};
+
+/* Pages, positions and cache slots of one step, from the requests' lengths.
+ * Request b has context[b] tokens in the cache, new_tokens[b] to add and owns
+ * owned[b] pages, block_table[b][0 .. owned[b]).  Requests are served in
+ * order: each takes the pages it lacks from the top of the stack
+ * free_pages[0 .. free_count).  A request that does not fit gets no page, but
+ * keeps its rows; status[b] says why:
+ *   0 planned
+ *   1 the free pages ran out at it (the pages that earlier unserved requests
+ *     lack count as taken, so the outcome does not depend on their sizes' order)
+ *   2 it needs more than table_width pages
+ *   3 its rows end past max_tokens
+ * Outputs: cu_new [requests + 1] (exclusive sums of new_tokens: request b's
+ * rows are cu_new[b] .. cu_new[b + 1]); seq_len[b] = context + new, 0 for an
+ * unserved request; owned_out[b] and free_count_out, the new state (each may
+ * be its input); the new pages in block_table (nothing else of it is
+ * written); for row t of request b, positions[t] and slots[t] =
+ * page * page_size + offset, -1 for the rows of an unserved request and for a
+ * page outside [0, pages).  Rows from cu_new[requests] to max_tokens get
+ * position 0 and slot -1.  Negative lengths count as 0.
+ * Limits: requests in [1, 8192], max_tokens and table_width < 2^31,
+ * pages * page_size < 2^31.  All pointers 4-byte aligned; only owned /
+ * owned_out and free_count / free_count_out may overlap. */
+typedef struct vvli_paged_plan_args {
+  uint64_t requests;
+  uint64_t page_size;
+  uint64_t pages;           /* entries of free_pages, and pages of the cache */
+  uint64_t table_width;     /* entries of a block_table row */
+  uint64_t max_tokens;      /* entries of positions and slots (0: neither is written) */
+  const int32_t* context;
+  const int32_t* new_tokens;
+  const int32_t* owned;
+  int32_t* block_table;     /* [requests][table_width] */
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* cu_new;
+  int32_t* seq_len;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* owned_out;
+  int32_t* free_count_out;
+  int32_t* status;
+} vvli_paged_plan_args;
+int vvli_cuda_paged_plan(int device, const vvli_paged_plan_args* args, void* stream);
+
+/* RMSNorm of q and k, rotary positions, and the cache write, in one pass:
+ *   y = x * w / sqrt(mean(x^2) + eps) over a head (VVLI_NORM_HEAD, w [head_dim])
+ *       or over all of the token's q (k) heads (VVLI_NORM_ROW, the OLMoE
+ *       qk_norm, src/llm.zig:45-48; w [heads][head_dim]), or x itself;
+ *   pair i < rotary_pairs of every head of y is turned by positions[t] *
+ *       inv_freq[i] radians (angle in 64 bits): elements i and
+ *       rotary_pairs + i, or 2 i and 2 i + 1 (interleaved; applyRoPE,
+ *       src/llm.zig:1337-1359); later elements are left;
+ *   q goes to q_out (which may be q), k and v (unnormed, unturned) to the
+ *       cache position slots[t] = page * page_size + offset.  A slot outside
+ *       the cache, -1 among them, writes no k and v.  Two rows with the same
+ *       slot leave either's values.
+ * Arithmetic in fp32, rounded once to the 16-bit type.
+ * Limits: head_dim a multiple of 16 in [16, 256], rotary_pairs a multiple of 8
+ * with 2 * rotary_pairs <= head_dim, q_heads and kv_heads in [1, 512], tokens <
+ * 2^31; strides (elements) multiples of 8 and at least a row; all 16-bit
+ * pointers 16-byte aligned.  tokens may be 0 (nothing is done). */
+enum vvli_qk_norm { VVLI_NORM_NONE = 0, VVLI_NORM_HEAD = 1, VVLI_NORM_ROW = 2 };
+typedef struct vvli_qk_rope_args {
+  uint64_t tokens;
+  uint64_t q_heads;
+  uint64_t kv_heads;
+  uint64_t head_dim;
+  uint64_t rotary_pairs;
+  uint64_t page_size;
+  uint64_t pages;
+  uint64_t page_stride;     /* elements between pages of a cache, at least kv_heads * page_size * head_dim */
+  uint64_t q_stride;        /* elements between tokens of q */
+  uint64_t k_stride;
+  uint64_t v_stride;
+  uint64_t out_stride;      /* elements between tokens of q_out */
+  int32_t dtype;            /* enum vvli_dtype, of everything 16-bit here */
+  int32_t norm;             /* enum vvli_qk_norm */
+  int32_t interleaved;      /* bool */
+  float eps;
+  const void* q;            /* [tokens][q_heads][head_dim] */
+  const void* k;            /* [tokens][kv_heads][head_dim] */
+  const void* v;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const void* q_weight;     /* norm weights; NULL: ones */
+  const void* k_weight;
+  const int32_t* positions; /* [tokens]; may be NULL when rotary_pairs is 0 */
+  const int32_t* slots;     /* [tokens] */
+  const double* inv_freq;   /* [rotary_pairs] */
+} vvli_qk_rope_args;
+int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* stream);
+
+/* Speculative sampling: verifies drafted tokens against the target's
+ * probabilities, with the random numbers given.  Request b has rows
+ * r0 = cu_rows[b] .. r1 = cu_rows[b + 1]; row r holds the token that was fed
+ * (tokens[r]) and the target's probabilities of the next one, so rows
+ * r0 + 1 .. r1 - 1 carry the drafts.  Draft i (tokens[r0 + i + 1]) is accepted
+ * while u_accept[r0 + i] * q < p, p = target[r0 + i][draft] and q =
+ * draft[r0 + i][draft] (1 without draft probabilities: a drafter that does not
+ * sample).  At the first rejection, row r, the token is drawn from
+ * max(0, target[r] - draft[r]) (from target[r] without the draft token when
+ * there are no draft probabilities; from target[r] if nothing is left); after
+ * the last draft from target[r1 - 1].  The draw is the smallest index whose
+ * cumulative weight exceeds u_sample[b] times the total, with weights and
+ * sums in 64 bits.  A draft outside [0, vocab) is rejected.
+ * Outputs: accepted[b]; out_tokens[r0 ..]: the accepted drafts, the drawn
+ * token, then -1 to r1.  Requests without rows get accepted 0; rows past
+ * cu_rows[requests] are left as they were.  NaN and negative weights count
+ * as 0.  Rows of probabilities need not sum to 1.
+ * Limits: requests in [1, 65535], vocab in [1, 2^30], strides (floats) >= vocab;
+ * cu_rows must not decrease and is cut at `rows`. */
+typedef struct vvli_verify_args {
+  uint64_t requests;
+  uint64_t rows;
+  uint64_t vocab;
+  uint64_t target_stride;
+  uint64_t draft_stride;
+  const float* target;      /* [rows][vocab] */
+  const float* draft;       /* [rows][vocab], or NULL */
+  const int32_t* tokens;    /* [rows] */
+  const int32_t* cu_rows;   /* [requests + 1] */
+  const float* u_accept;    /* [rows] */
+  const float* u_sample;    /* [requests] */
+  int32_t* accepted;        /* [requests] */
+  int32_t* out_tokens;      /* [rows] */
+} vvli_verify_args;
+int vvli_cuda_verify_drafts(int device, const vvli_verify_args* args, void* stream);
+
 /* Device-side timing of the last forward in milliseconds (CUDA events). */
 int vvli_cuda_last_forward_ms(vvli_ctx* ctx, float* out_ms);
 

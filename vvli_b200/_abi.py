@@ -66,6 +66,32 @@ class CMoeArgs(ctypes.Structure):
     ]
 
 
+class CPagedPlanArgs(ctypes.Structure):
+    """vvli_paged_plan_args (include/vvli_cuda.h)."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("requests", "page_size", "pages", "table_width", "max_tokens")] + [
+        (n, ctypes.c_void_p) for n in ("context", "new_tokens", "owned", "block_table", "free_pages", "free_count",
+                                       "cu_new", "seq_len", "positions", "slots", "owned_out", "free_count_out",
+                                       "status")]
+
+
+class CQkRopeArgs(ctypes.Structure):
+    """vvli_qk_rope_args (include/vvli_cuda.h)."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("tokens", "q_heads", "kv_heads", "head_dim", "rotary_pairs", "page_size",
+                                               "pages", "page_stride", "q_stride", "k_stride", "v_stride",
+                                               "out_stride")] + [
+        ("dtype", ctypes.c_int32), ("norm", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "q_weight", "k_weight",
+                                       "positions", "slots", "inv_freq")]
+
+
+class CVerifyArgs(ctypes.Structure):
+    """vvli_verify_args (include/vvli_cuda.h)."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("requests", "rows", "vocab", "target_stride", "draft_stride")] + [
+        (n, ctypes.c_void_p) for n in ("target", "draft", "tokens", "cu_rows", "u_accept", "u_sample", "accepted",
+                                       "out_tokens")]
+
+
 # name -> (restype, argtypes); every function declared in include/vvli_cuda.h.
 SIGNATURES = {
     "vvli_cuda_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -107,6 +133,9 @@ SIGNATURES = {
     "vvli_cuda_debug_hidden": (ctypes.c_int, [_ctx, ctypes.c_int, _f32p]),
     "vvli_cuda_moe_workspace_bytes": (ctypes.c_uint64, [ctypes.c_uint64] * 5),
     "vvli_cuda_moe_ffn": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CMoeArgs), ctypes.c_void_p]),
+    "vvli_cuda_paged_plan": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CPagedPlanArgs), ctypes.c_void_p]),
+    "vvli_cuda_qk_rope_write": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CQkRopeArgs), ctypes.c_void_p]),
+    "vvli_cuda_verify_drafts": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CVerifyArgs), ctypes.c_void_p]),
     "vvli_cuda_last_forward_ms": (ctypes.c_int, [_ctx, _f32p]),
     "vvli_cuda_destroy": (ctypes.c_int, [_ctx]),
 }
