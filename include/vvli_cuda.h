@@ -494,16 +494,17 @@ enum vvli_dtype {
  * unserved request; owned_out[b] and free_count_out, the new state (each may
  * be its input); the new pages in block_table (nothing else of it is
  * written); for row t of request b, positions[t] and slots[t] =
- * page * page_size + offset, -1 for the rows of an unserved request and for a
- * page outside [0, pages).  Rows from cu_new[requests] to max_tokens get
+ * page * page_size + offset, -1 for the rows of an unserved request and where
+ * the table (or the stack) holds no page (a negative entry, or a slot that
+ * would not fit).  Rows from cu_new[requests] to max_tokens get
  * position 0 and slot -1.  Negative lengths count as 0.
  * Limits: requests in [1, 8192], max_tokens and table_width < 2^31,
- * pages * page_size < 2^31.  All pointers 4-byte aligned; only owned /
+ * free_entries in [1, 2^31).  All pointers 4-byte aligned; only owned /
  * owned_out and free_count / free_count_out may overlap. */
 typedef struct vvli_paged_plan_args {
   uint64_t requests;
   uint64_t page_size;
-  uint64_t pages;           /* entries of free_pages, and pages of the cache */
+  uint64_t free_entries;    /* entries of free_pages */
   uint64_t table_width;     /* entries of a block_table row */
   uint64_t max_tokens;      /* entries of positions and slots (0: neither is written) */
   const int32_t* context;
@@ -570,6 +571,64 @@ typedef struct vvli_qk_rope_args {
   const double* inv_freq;   /* [rotary_pairs] */
 } vvli_qk_rope_args;
 int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* stream);
+
+/* Attention of every request's new tokens over its paged cache (the new
+ * tokens' own k and v already written).  Row cu_new[b] + i of q is request b's
+ * position p = seq_len[b] - (cu_new[b + 1] - cu_new[b]) + i and sees the keys
+ * at positions j <= p, with window > 0 only those with j > p - window:
+ *   s_j = scale * q . k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);
+ *   alibi: s_j += alibi[head] * (j - p);  out = sum_j softmax(s)_j v_j,
+ *   lse = ln(sum_j exp(s_j)).
+ * q head g uses kv head g / (q_heads / kv_heads).  A row that sees no key
+ * (p < 0) gets out 0 and lse -inf; rows from cu_new[requests] on are left as
+ * they were.  What the cache holds past a request's seq_len is never used,
+ * whatever its bits.  Keys whose table entry is outside [0, pages), or past
+ * table_width, count as zero keys and values.  cu_new must not decrease and
+ * is cut at `tokens`.  Products of 16-bit values summed in fp32; the
+ * probabilities enter the second product rounded to the 16-bit type, relative
+ * to the row's largest score; results do not depend on timing.
+ * `max_new` is the longest request's new tokens as far as the caller knows:
+ * it picks the kernel, not the result (up to a rounding).  A call queues two
+ * kernels.  Two calls that may run at the same time need a workspace each.
+ * Limits: head_dim 64 or 128; q_heads a multiple of kv_heads, q_heads <= 512;
+ * tokens * q_heads < 2^31; requests in [1, 65536]; window < 2^31; strides (elements) multiples of 8 and at least a
+ * row; 16-bit pointers 16-byte aligned; workspace 256-byte aligned.  The first
+ * int32 of the workspace is set to VVLI_ERR_TIMEOUT if a bounded wait gave up
+ * (never cleared; zero it before the first call to read it). */
+typedef struct vvli_paged_attn_args {
+  uint64_t requests;
+  uint64_t tokens;          /* rows of q and out */
+  uint64_t q_heads;
+  uint64_t kv_heads;
+  uint64_t head_dim;
+  uint64_t page_size;
+  uint64_t pages;
+  uint64_t page_stride;     /* elements between pages of a cache */
+  uint64_t table_width;     /* entries of a block_table row */
+  uint64_t q_stride;        /* elements between rows of q */
+  uint64_t out_stride;
+  uint64_t max_new;
+  uint64_t window;          /* 0: none */
+  int32_t dtype;            /* enum vvli_dtype */
+  float scale;
+  float softcap;            /* 0: none */
+  uint32_t _pad0;
+  const void* q;            /* [tokens][q_heads][head_dim] */
+  const void* k_cache;
+  const void* v_cache;
+  void* out;                /* [tokens][q_heads][head_dim] */
+  float* lse;               /* [tokens][q_heads], or NULL */
+  const float* alibi;       /* [q_heads], or NULL */
+  const int32_t* block_table; /* [requests][table_width] */
+  const int32_t* cu_new;    /* [requests + 1] */
+  const int32_t* seq_len;   /* [requests] */
+  void* workspace;
+  uint64_t workspace_bytes;
+} vvli_paged_attn_args;
+
+/* Workspace bytes vvli_cuda_paged_attention needs, whatever the lengths; 0 for a head_dim it does not take. */
+uint64_t vvli_cuda_paged_attn_workspace_bytes(uint64_t head_dim);
+int vvli_cuda_paged_attention(int device, const vvli_paged_attn_args* args, void* stream);
 
 /* Speculative sampling: verifies drafted tokens against the target's
  * probabilities, with the random numbers given.  Request b has rows

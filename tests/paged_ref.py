@@ -5,11 +5,11 @@ import math
 import torch
 
 
-def plan(context, new, owned, table, free_pages, free_count, page, pages, max_tokens):
+def plan(context, new, owned, table, free_pages, free_count, page, max_tokens):
     """What vvli_cuda_paged_plan documents, request by request; table is changed in place."""
     cu, seq, own, status, pos, slot = [0], [], [], [], [0] * max_tokens, [-1] * max_tokens
     lacking = taken = 0
-    free = min(max(0, free_count), pages)
+    free = min(max(0, free_count), len(free_pages))
     for b, (c, n, o) in enumerate(zip(context, new, owned)):
         c, n, o = max(0, c), max(0, n), max(0, o)
         row = cu[-1]
@@ -27,7 +27,7 @@ def plan(context, new, owned, table, free_pages, free_count, page, pages, max_to
                 pos[row + i] = c + i
                 if st == 0:
                     at = table[b][(c + i) // page]
-                    slot[row + i] = at * page + (c + i) % page if 0 <= at < pages else -1
+                    slot[row + i] = at * page + (c + i) % page if 0 <= at <= (2**31 - page) // page else -1
         seq.append(0 if st else c + n)
         own.append(o + need)
         status.append(st)

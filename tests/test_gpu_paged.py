@@ -37,7 +37,7 @@ def make_plan(seed, B, page, ctx, new, spare, width_slack=1, over=0):
     for o in owned:
         table.append(ids[at:at + o] + [-7] * (width - o))
         at += o
-    free = ids[at:] + [-9] * (pages - (len(ids) - at))
+    free = ids[at:] + [-9] * 3
     return context, news, owned, table, free, max(0, need + spare), page, pages
 
 
@@ -48,7 +48,7 @@ def check_plan(torch, case, max_tokens, inplace=False):
     own, cnt = ints(torch, owned), ints(torch, [count])
     p = plan_step(ints(torch, context), ints(torch, new), own, tab, ints(torch, free), cnt, page, max_tokens,
                   inplace=inplace)
-    want = ref.plan(context, new, owned, table, free, count, page, pages, max_tokens)
+    want = ref.plan(context, new, owned, table, free, count, page, max_tokens)
     for name, w in zip(p._fields, want):
         assert getattr(p, name).tolist() == w, name
     assert tab.tolist() == table
@@ -77,7 +77,7 @@ def test_plan_refused_requests(torch):
     case = list(make_plan(8, 40, 16, 200, 50, spare=30, width_slack=0))
     case[0][3] = 16 * len(case[3][0]) + 1
     case[1][4], case[0][5], case[2][6] = -3, -1, -5
-    case[3][7][0], case[3][8][0] = -1, case[7]
+    case[3][7][0], case[3][8][0], case[3][9][0] = -1, 2**31 - 1, 2**27 - 1
     want = check_plan(torch, tuple(case), sum(max(0, n) for n in case[1]) - 60)
     assert {0, 2, 3} <= set(want[6])
     check_plan(torch, make_plan(9, 3, 64, 10, 10, spare=0), 0)  # no rows wanted
@@ -256,7 +256,7 @@ def test_plan_and_write_captured_on_another_stream(torch):
         c.zero_()
     graph.replay()
     torch.cuda.synchronize()
-    want = ref.plan(context, new2, owned, table, free, count, page, pages, rows)
+    want = ref.plan(context, new2, owned, table, free, count, page, rows)
     for name, w in zip(p._fields, want):
         assert getattr(p, name).tolist() == w, name
     for t, s in enumerate(want[3]):

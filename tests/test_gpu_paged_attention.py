@@ -1,0 +1,273 @@
+"""vvli_cuda_paged_attention against a plain implementation in 64 bits.  Needs a B200."""
+
+import math
+import random
+
+import pytest
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+def make(torch, seed, lens, hq, hk, d, page, dtype, poison=True, spread=1.5, bad_pages=(), extra_rows=0, width_slack=2):
+    """lens: (seq_len, new tokens) of each request. Cells of the cache past a request's end hold NaN and infinities."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-max(0, e) // page) for e, _ in lens]
+    pages = sum(need) + 3
+    order = torch.randperm(pages, generator=g).tolist()
+    width = max(need + [1]) + width_slack
+    table, at = [], 0
+    for n in need:
+        table.append(order[at:at + n] + [-1] * (width - n))
+        at += n
+    k, v = (torch.randn(pages, hk, page, d, generator=g).to(dtype) for _ in range(2))
+    if poison:
+        for c, fill in ((k, math.nan), (v, math.inf)):
+            spare = torch.ones(pages, page, dtype=torch.bool)
+            for b, (e, _) in enumerate(lens):
+                for j in range(need[b]):
+                    spare[table[b][j], :min(page, e - j * page)] = False
+            c.transpose(1, 2)[spare] = fill
+    for b, j, value in bad_pages:
+        table[b][j] = value
+    T = sum(n for _, n in lens)
+    q = (torch.randn(T + extra_rows, hq, d, generator=g) * spread).to(dtype)
+    cu = [sum(n for _, n in lens[:i]) for i in range(len(lens) + 1)]
+    return q, k, v, table, cu, [e for e, _ in lens]
+
+
+def check(torch, inp, page, max_new=None, window=0, softcap=0.0, alibi=None, scale=None, att=None):
+    from vvli_b200.paged import PagedAttention
+    q, k, v, table, cu, seq = inp
+    T, hq, d = q.shape
+    hk, dtype = k.shape[1], q.dtype
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    if att is None:
+        att = PagedAttention(hq, hk, d, page, dtype=dtype, scale=scale, softcap=softcap, window=window,
+                             alibi=None if alibi is None else alibi.cuda())
+    out = torch.full((T, hq, d), 7.0, dtype=dtype, device="cuda")
+    lse = torch.full((T, hq), 7.0, device="cuda")
+    longest = max(b - a for a, b in zip(cu, cu[1:]))
+    att(q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), longest if max_new is None else max_new, out=out,
+        lse=lse)
+    torch.cuda.synchronize()
+    assert att.status() == 0
+    want, wlse = ref.attention(q, k, v, table, cu, seq, d**-0.5 if scale is None else scale, window, softcap, alibi)
+    rows = ~torch.isnan(wlse).any(-1)
+    out, lse = out.cpu(), lse.cpu()
+    assert bool((out[~rows] == 7).all()) and bool((lse[~rows] == 7).all())  # rows of no request
+    got, want, lse, wlse = out[rows].double(), want[rows], lse[rows].double(), wlse[rows]
+    empty = torch.isinf(wlse)
+    assert torch.equal(empty, lse == -math.inf) and bool((got[empty] == 0).all())
+    # Scores: 16-bit products are exact in fp32, sums of up to 128 of them stay within
+    # 2^-21 of the sum of their magnitudes (at most 2^9 in these tests): a score is off
+    # by less than 2^-12, with the exponential a probability and the sum of them by 2^-11.
+    # Probabilities and output are rounded to the type: half a step each, of a weighted
+    # mean of values (at most the largest |v|).
+    half = torch.finfo(dtype).eps / 2
+    big = torch.nan_to_num(v.double(), 0.0, 0.0, 0.0).abs().max()
+    tol = half * want.abs() + (half + 2.0**-10) * big
+    bad = (got - want).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), float(((got - want).abs() / tol).max()))
+    # and on the whole: the errors of many keys average out (root mean square of a rounding: 1/sqrt(3) of half a step)
+    if got.numel() > 5000:
+        assert float((got - want).norm() / want.norm()) < 2 * half
+    fine = ~empty
+    assert bool(((lse - wlse)[fine].abs() <= 2.0**-10).all())
+    return out
+
+
+HEADS = [(14, 2, 64), (32, 8, 128), (4, 4, 128), (8, 1, 64), (3, 1, 128), (40, 2, 64)]
+
+
+@pytest.mark.parametrize("hq,hk,d", HEADS)
+@pytest.mark.parametrize("page,dtype", [(16, "bfloat16"), (32, "float16"), (64, "bfloat16"), (128, "float16")])
+def test_decode(torch, hq, hk, d, page, dtype):
+    lens = [(1, 1), (16, 1), (17, 1), (63, 1), (64, 1), (65, 1), (129, 1), (500, 1), (0, 0), (1000, 1), (2, 1)]
+    check(torch, make(torch, d + page, lens, hq, hk, d, page, getattr(torch, dtype)), page)
+
+
+@pytest.mark.parametrize("hq,hk,d", HEADS)
+@pytest.mark.parametrize("n", [2, 5, 9, 33])
+def test_drafts(torch, hq, hk, d, n):
+    lens = [(n, n), (n + 1, n), (64 + n // 2, n), (130, n), (700, n), (65, 1), (300, max(1, n - 1))]
+    check(torch, make(torch, n + hq, lens, hq, hk, d, 16 if n % 2 else 64, torch.bfloat16), 16 if n % 2 else 64)
+
+
+@pytest.mark.parametrize("hq,hk,d,page,dtype", [(14, 2, 64, 16, "float16"), (32, 8, 128, 64, "bfloat16"),
+                                                (4, 4, 128, 128, "bfloat16"), (6, 1, 64, 32, "bfloat16")])
+def test_chunks(torch, hq, hk, d, page, dtype):
+    lens = [(300, 300), (257, 100), (1, 1), (128, 128), (129, 129), (600, 129), (511, 1), (90, 64), (1000, 65)]
+    check(torch, make(torch, d, lens, hq, hk, d, page, getattr(torch, dtype)), page)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 200, 5000])
+@pytest.mark.parametrize("long", [False, True])
+def test_window(torch, window, long):
+    lens = [(300, 130), (200, 70), (129, 129)] if long else [(300, 3), (1, 1), (129, 4), (900, 2)]
+    check(torch, make(torch, window, lens, 8, 2, 64, 32, torch.bfloat16), 32, window=window)
+
+
+@pytest.mark.parametrize("softcap,with_alibi,window", [(30.0, False, 0), (0.0, True, 0), (5.0, True, 100), (50.0, False, 64)])
+@pytest.mark.parametrize("long", [False, True])
+def test_softcap_and_alibi(torch, softcap, with_alibi, window, long):
+    alibi = torch.tensor([2.0**-i for i in range(1, 9)]) if with_alibi else None
+    lens = [(300, 150), (140, 140), (80, 1)] if long else [(300, 3), (1, 1), (129, 4), (900, 2)]
+    for d, dtype in ((64, torch.float16), (128, torch.bfloat16)):
+        check(torch, make(torch, 5, lens, 8, 2, d, 64, dtype, spread=4.0), 64, softcap=softcap, alibi=alibi, window=window)
+
+
+@pytest.mark.parametrize("max_new", [0, 1, 4, 300, 10**6])
+def test_max_new_only_picks_the_kernel(torch, max_new):
+    lens = [(300, 120), (64, 1), (200, 7), (33, 33)]
+    check(torch, make(torch, 2, lens, 8, 2, 128, 64, torch.bfloat16), 64, max_new=max_new)
+
+
+@pytest.mark.parametrize("max_new", [1, 10**6])
+def test_empty_rows_bad_pages_and_rows_behind(torch, max_new):
+    # seq_len 0 (an unserved request), fewer keys than rows, entries outside the cache, a short table
+    lens = [(0, 3), (2, 5), (-4, 2), (100, 4), (200, 1), (150, 2)]
+    inp = list(make(torch, 3, lens, 4, 2, 64, 16, torch.bfloat16, extra_rows=5,
+                    bad_pages=[(3, 1, -1), (4, 0, 10**9), (4, 5, -2**31), (5, 2, 2**31 - 1)], width_slack=0))
+    check(torch, tuple(inp), 16, max_new=max_new)
+    inp[3] = [r[:9] for r in inp[3]]  # request 4 and 5 need 13 and 10 entries
+    check(torch, tuple(inp), 16, max_new=max_new)
+    check(torch, make(torch, 3, [(0, 0), (0, 0)], 4, 2, 64, 16, torch.bfloat16, extra_rows=2), 16, max_new=max_new)
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_cut_rows(torch, long):
+    # cu_new past the rows of q: the rows there are keep their positions
+    n = 200 if long else 4
+    q, k, v, table, cu, seq = make(torch, 4, [(n + 40, n), (n + 3, n)], 4, 2, 64, 16, torch.float16)
+    check(torch, (q[:n + n // 2].contiguous(), k, v, table, cu, seq), 16)
+    check(torch, (q[:n - 2].contiguous(), k, v, table, cu, seq), 16)
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_strides(torch, long):
+    from vvli_b200.paged import PagedAttention
+    n = 140 if long else 2
+    lens = [(200, n), (n, n), (333, n)]
+    q, k, v, table, cu, seq = make(torch, 6, lens, 8, 2, 128, 32, torch.bfloat16)
+    want = check(torch, (q, k, v, table, cu, seq), 32)
+    both = torch.stack([k, v], 1).cuda()  # pages of keys and values side by side
+    wide = torch.randn(q.shape[0], 1600).to(q.dtype).cuda()
+    wide[:, 8:8 + 1024] = q.cuda().view(-1, 1024)
+    res = torch.zeros(q.shape[0], 1040, dtype=q.dtype, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    PagedAttention(8, 2, 128, 32)(wide[:, 8:8 + 1024].view(-1, 8, 128), both[:, 0], both[:, 1], ints(table), ints(cu),
+                                  ints(seq), n, out=res[:, 16:].view(-1, 8, 128))
+    assert torch.equal(res[:, 16:].cpu().view(-1, 8, 128), want) and bool((res[:, :16] == 0).all())
+
+
+@pytest.mark.parametrize("lens", [[(40000, 1)], [(20000, 4), (5, 1)], [(9000, 40)], [(3000, 1500)],
+                                  [(100 + 37 * i % 900, 1) for i in range(700)],
+                                  [(1 + 7 * i % 50, 1 + 7 * i % 50) for i in range(40)]])
+def test_split_over_ctas(torch, lens):
+    # one request over all SMs, many over each SM, and items that end inside shares
+    check(torch, make(torch, 7, lens, 4, 1, 64, 64, torch.bfloat16, poison=False), 64)
+
+
+def test_large_scores_and_fully_peaked_rows(torch):
+    for lens in ([(500, 2)], [(500, 200)]):
+        q, k, v, table, cu, seq = make(torch, 8, lens, 4, 2, 64, 16, torch.float16, spread=20.0)
+        check(torch, (q, k, v, table, cu, seq), 16, scale=0.25)
+        check(torch, (q, k, v, table, cu, seq), 16, scale=0.0)
+        check(torch, (q, k, v, table, cu, seq), 16, scale=-0.125)
+
+
+def test_infinite_and_nan_keys_in_sight_reach_the_row(torch):
+    # what a row sees is not masked: a NaN value gives NaN in its column, a +inf score NaN in the row, as the formula
+    from vvli_b200.paged import PagedAttention
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for new, max_new in ((1, 1), (130, 130)):
+        q, k, v, table, cu, seq = make(torch, 9, [(200, new), (150, new)], 4, 2, 64, 16, torch.bfloat16, poison=False)
+        v[table[0][1], 0, 3, 5] = math.nan
+        out = PagedAttention(4, 2, 64, 16)(q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), max_new).cpu()
+        nan = torch.isnan(out)
+        assert bool(nan[:new, :2, 5].all()) and int(nan.sum()) == 2 * new
+
+
+def test_offsets_past_32_bits(torch):
+    # pages whose element offset passes 2^32, in caches of one request's pages far apart
+    from vvli_b200.paged import PagedAttention
+    hk, page, d = 2, 16, 128
+    stride = 1 << 29
+    base = torch.zeros(stride * 9, dtype=torch.bfloat16, device="cuda")
+    cache = base.as_strided((9, hk, page, d), (stride, page * d, d, 1))
+    k = torch.randn(9, hk, page, d).to(torch.bfloat16)
+    cache.copy_(k.cuda())
+    table = [[8, 0, 7, 3, 5, 6, 1, 2, 4]]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for n in (1, 40):
+        q = torch.randn(n, 4, d).to(torch.bfloat16)
+        out = PagedAttention(4, hk, d, page)(q.cuda(), cache, cache, ints(table), ints([0, n]), ints([141]), n)
+        want, _ = ref.attention(q, k, k, table, [0, n], [141], d**-0.5)
+        assert float((out.cpu().double() - want).norm() / want.norm()) < 2.0**-7
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_repeats_bit_for_bit_captured_and_on_another_stream(torch, new):
+    from vvli_b200.paged import PagedAttention
+    r = random.Random(1)
+    lens = [(new + r.randint(0, 600), new) for _ in range(6)]
+    q, k, v, table, cu, seq = make(torch, 10, lens, 8, 2, 128, 64, torch.bfloat16)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    att = PagedAttention(8, 2, 128, 64)
+    args = (q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), new)
+    first, l1 = att(*args, lse=True)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    second = att(*args, stream=side)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        third, l3 = att(*args, lse=True)
+    for _ in range(2):
+        third.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(third, first) and torch.equal(l3, l1)
+    assert torch.equal(second, first)
+    # the captured call serves other lengths of the same batch
+    seq2 = [max(new, s - 50) for s in seq]
+    args[5].copy_(ints(seq2))
+    graph.replay()
+    torch.cuda.synchronize()
+    want, _ = ref.attention(q, torch.nan_to_num(k, 0.0), torch.nan_to_num(v, 0.0, 0.0, 0.0), table, cu, seq2, 128**-0.5)
+    assert float((third.cpu().double() - want).norm() / want.norm()) < 2.0**-7
+
+
+def test_wrapper_refusals(torch):
+    from vvli_b200.errors import VvliError
+    from vvli_b200.paged import PagedAttention
+    with pytest.raises(ValueError):
+        PagedAttention(4, 2, 96, 16)
+    with pytest.raises(ValueError):
+        PagedAttention(4, 2, 64, 16, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        PagedAttention(4, 2, 64, 16, alibi=torch.zeros(3, device="cuda"))
+    att = PagedAttention(4, 2, 64, 16)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    q, c, t = z(3, 4, 64), z(5, 2, 16, 64), i.view(2, 2)
+    for bad in (lambda: att(q.half(), c, c, t, i[:3], i[:2], 1), lambda: att(z(3, 2, 64), c, c, t, i[:3], i[:2], 1),
+                lambda: att(q, z(5, 2, 32, 64), z(5, 2, 32, 64), t, i[:3], i[:2], 1),
+                lambda: att(q, c, c[:4], t, i[:3], i[:2], 1), lambda: att(q, c, c, t[:1], i[:3], i[:2], 1),
+                lambda: att(q, c, c, t, i[:2], i[:2], 1), lambda: att(q, c, c, t.long(), i[:3], i[:2], 1),
+                lambda: att(q, c, c, t, i[:3], i[:2], 1, out=z(2, 4, 64)),
+                lambda: att(q, c, c, t, i[:3], i[:2], 1, lse=torch.zeros(3, 3, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(VvliError):
+        PagedAttention(5, 2, 64, 16)(z(3, 5, 64), c, c, t, i[:3], i[:2], 1)
+    assert att(q[:0], c, c, t, i[:3], i[:2], 1).shape == (0, 4, 64)

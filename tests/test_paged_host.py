@@ -23,6 +23,7 @@ def test_struct_layouts():
     assert ctypes.sizeof(_abi.CPagedPlanArgs) == (5 + 13) * 8
     assert ctypes.sizeof(_abi.CQkRopeArgs) == 12 * 8 + 4 * 4 + 11 * 8 and _abi.CQkRopeArgs.q.offset == 112
     assert ctypes.sizeof(_abi.CVerifyArgs) == (5 + 8) * 8
+    assert ctypes.sizeof(_abi.CPagedAttnArgs) == 13 * 8 + 4 * 4 + 11 * 8 and _abi.CPagedAttnArgs.q.offset == 120
 
 
 def test_plan_refusals():
@@ -31,7 +32,7 @@ def test_plan_refusals():
     assert fn(0, None, None) == INVALID
     for changes, text in (
             ({"requests": 0}, "requests"), ({"requests": 8193}, "requests"), ({"page_size": 48}, "page_size"),
-            ({"page_size": 256}, "page_size"), ({"pages": 0}, "pages"), ({"pages": 1 << 26}, "pages"),
+            ({"page_size": 256}, "page_size"), ({"free_entries": 0}, "free_entries"), ({"free_entries": 1 << 31}, "free_entries"),
             ({"table_width": 0}, "table_width"), ({"table_width": 1 << 31}, "table_width"),
             ({"max_tokens": 1 << 31}, "max_tokens"), ({"context": None}, "null"), ({"status": None}, "null"),
             ({"slots": None}, "null"), ({"positions": PTR + 2}, "aligned"), ({"cu_new": PTR + 1}, "aligned")):
@@ -52,6 +53,30 @@ def test_qk_refusals():
             ({"eps": float("nan")}, "eps"), ({"q": None}, "null"), ({"v_cache": None}, "null"), ({"slots": None}, "null"),
             ({"positions": None}, "null"), ({"inv_freq": None}, "null"), ({"k": PTR + 8}, "aligned"),
             ({"k_weight": PTR + 2}, "aligned"), ({"inv_freq": PTR + 4}, "aligned")):
+        refused(fn, good, changes, text)
+
+
+def test_attention_refusals_and_workspace():
+    lib = _abi.lib()
+    assert lib.vvli_cuda_paged_attn_workspace_bytes(96) == 0
+    small, large = (lib.vvli_cuda_paged_attn_workspace_bytes(d) for d in (64, 128))
+    assert 0 < small < large < 64 << 20
+    fn = lib.vvli_cuda_paged_attention
+    good = _abi.CPagedAttnArgs(4, 9, 14, 2, 64, 16, 10, 2 * 16 * 64, 5, 14 * 64, 14 * 64, 3, 0, 0, 0.125, 0.0, 0,
+                               *[PTR] * 10, small)
+    assert fn(0, None, None) == INVALID
+    for changes, text in (
+            ({"requests": 0}, "requests"), ({"requests": 65537}, "requests"), ({"head_dim": 96}, "head_dim"),
+            ({"q_heads": 15}, "q_heads"), ({"q_heads": 514}, "q_heads"), ({"kv_heads": 0}, "q_heads"),
+            ({"tokens": (1 << 31) // 14 + 1}, "tokens"), ({"page_size": 24}, "page_size"), ({"pages": 0}, "pages"),
+            ({"pages": 1 << 27}, "pages"), ({"page_stride": 2 * 16 * 64 + 2}, "page_stride"),
+            ({"page_stride": 16 * 64}, "page_stride"), ({"table_width": 0}, "table_width"),
+            ({"q_stride": 13 * 64}, "strides"), ({"out_stride": 14 * 64 + 4}, "strides"),
+            ({"window": 1 << 31}, "window"), ({"dtype": 2}, "dtype"), ({"scale": float("inf")}, "scale"),
+            ({"softcap": -1.0}, "softcap"), ({"softcap": float("nan")}, "softcap"), ({"q": None}, "null"),
+            ({"workspace": None}, "null"), ({"seq_len": None}, "null"), ({"v_cache": PTR + 8}, "aligned"),
+            ({"lse": PTR + 2}, "aligned"), ({"workspace": PTR + 128}, "workspace"),
+            ({"workspace_bytes": small - 1}, "workspace_bytes")):
         refused(fn, good, changes, text)
 
 

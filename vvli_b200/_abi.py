@@ -68,7 +68,8 @@ class CMoeArgs(ctypes.Structure):
 
 class CPagedPlanArgs(ctypes.Structure):
     """vvli_paged_plan_args (include/vvli_cuda.h)."""
-    _fields_ = [(n, ctypes.c_uint64) for n in ("requests", "page_size", "pages", "table_width", "max_tokens")] + [
+    _fields_ = [(n, ctypes.c_uint64) for n in ("requests", "page_size", "free_entries", "table_width",
+                                               "max_tokens")] + [
         (n, ctypes.c_void_p) for n in ("context", "new_tokens", "owned", "block_table", "free_pages", "free_count",
                                        "cu_new", "seq_len", "positions", "slots", "owned_out", "free_count_out",
                                        "status")]
@@ -83,6 +84,17 @@ class CQkRopeArgs(ctypes.Structure):
         ("eps", ctypes.c_float)] + [
         (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "q_weight", "k_weight",
                                        "positions", "slots", "inv_freq")]
+
+
+class CPagedAttnArgs(ctypes.Structure):
+    """vvli_paged_attn_args (include/vvli_cuda.h)."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("requests", "tokens", "q_heads", "kv_heads", "head_dim", "page_size",
+                                               "pages", "page_stride", "table_width", "q_stride", "out_stride",
+                                               "max_new", "window")] + [
+        ("dtype", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("_pad0", ctypes.c_uint32)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "lse", "alibi", "block_table", "cu_new",
+                                       "seq_len", "workspace")] + [("workspace_bytes", ctypes.c_uint64)]
 
 
 class CVerifyArgs(ctypes.Structure):
@@ -135,6 +147,8 @@ SIGNATURES = {
     "vvli_cuda_moe_ffn": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CMoeArgs), ctypes.c_void_p]),
     "vvli_cuda_paged_plan": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CPagedPlanArgs), ctypes.c_void_p]),
     "vvli_cuda_qk_rope_write": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CQkRopeArgs), ctypes.c_void_p]),
+    "vvli_cuda_paged_attn_workspace_bytes": (ctypes.c_uint64, [ctypes.c_uint64]),
+    "vvli_cuda_paged_attention": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CPagedAttnArgs), ctypes.c_void_p]),
     "vvli_cuda_verify_drafts": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(CVerifyArgs), ctypes.c_void_p]),
     "vvli_cuda_last_forward_ms": (ctypes.c_int, [_ctx, _f32p]),
     "vvli_cuda_destroy": (ctypes.c_int, [_ctx]),

@@ -1,0 +1,349 @@
+// paged_attn.cuh - what the two kernels of vvli_cuda_paged_attention share: the
+// work schedule, the split parts and the score arithmetic.
+//
+// Work.  A request's query rows of one kv head are packed: row r is the new
+// token r / G and the group's q head r % G.  An item is (request, kv head,
+// block of ROWS packed rows); its units are the KT-key tiles that any of its
+// rows sees.  The units of all items in order (request, head, block, tile)
+// form one line that is cut into equal shares, one per CTA, whatever the
+// lengths: a CTA's share is a run of segments, each a range of one item's
+// tiles.  A segment that is a whole item writes its output; the others (at most
+// the first and the last of a CTA) leave unnormalised sums and their running
+// maximum in the workspace, two slots per CTA, and the combine kernel adds an
+// item's parts in tile order.  The lengths stay on the device: every CTA sums
+// the units over the requests for itself.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "common.cuh"
+#include "op_common.cuh"
+
+namespace vvli {
+
+constexpr int kPaMaxCtas = 160;    // CTAs of a launch at most: the workspace is sized for them
+constexpr int kPaMaxRows = 256;    // rows of an item at most
+
+struct PaDesc {  // what the combine kernel needs of a CTA
+  int finish;    // its first segment ends an item that another CTA began
+  int b, h, blk;
+  int active;    // CTAs with a share
+  int pad;
+  long long item_first;  // first unit of that item
+  long long total;       // units of the call
+};
+
+struct PaParams {
+  int B, T, hq, hk, G, shift, pages, width;  // page_size = 1 << shift
+  int window;                                // 0: none
+  float scale_log2;                          // scale * log2(e)
+  float cap_in, cap_log2;                    // softcap: scale / cap * 2 log2(e); cap * log2(e); 0 without
+  long long q_stride, out_stride;
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse;
+  const float* alibi;
+  const int *table, *cu, *seq;
+  // workspace
+  int* err;
+  PaDesc* desc;    // [kPaMaxCtas]
+  float* part_ml;  // [kPaMaxCtas][2][kPaMaxRows][2] running maximum (log2 units) and sum
+  float* part_o;   // [kPaMaxCtas][2][rows of an item][D]
+};
+
+inline size_t pa_workspace_bytes(int d) {
+  const size_t slots = static_cast<size_t>(kPaMaxCtas) * 2 * kPaMaxRows;
+  return 256 + kPaMaxCtas * sizeof(PaDesc) + slots * 2 * sizeof(float) + slots * d * sizeof(float);
+}
+
+// ---------------------------------------------------------------- schedule
+
+struct PaReq {
+  int row0;  // first row of q
+  int n;     // rows of q (tokens)
+  int pos0;  // position of the first (may be negative)
+};
+
+VVLI_DEV PaReq pa_request(const PaParams& p, int b) {
+  const int c0 = min(max(p.cu[b], 0), p.T), c1 = max(p.cu[b + 1], c0);
+  PaReq r;
+  r.row0 = c0;
+  r.n = min(c1, p.T) - c0;
+  // lengths that no cache holds are cut, so that positions and tiles stay in 32 bits
+  r.pos0 = max(min(p.seq[b], INT_MAX - 1024), 0) - (c1 - c0);
+  return r;
+}
+
+template <int ROWS>
+VVLI_DEV int pa_blocks(const PaParams& p, const PaReq& r) {
+  return (r.n * p.G + ROWS - 1) / ROWS;
+}
+
+// Keys [lo, hi) that rows of block blk see, and its tiles [t0, t1), one at least.
+struct PaItem {
+  int rows;     // rows of the block
+  int lo, hi;
+  int t0, t1;
+};
+template <int ROWS, int KT>
+VVLI_DEV PaItem pa_item(const PaParams& p, const PaReq& r, int blk) {
+  PaItem it;
+  it.rows = min(ROWS, r.n * p.G - blk * ROWS);
+  const int first = r.pos0 + blk * ROWS / p.G, last = r.pos0 + (blk * ROWS + it.rows - 1) / p.G;
+  it.hi = max(0, last + 1);
+  it.lo = p.window && first >= p.window ? first + 1 - p.window : 0;
+  it.t0 = it.lo / KT;
+  it.t1 = max(it.t0 + 1, (it.hi + KT - 1) / KT);
+  return it;
+}
+
+struct PaShare {
+  long long total, u0, u1;  // units of the call; this CTA's
+  int active;               // CTAs with a share
+  int b, h, blk, off;       // where u0 lies: item and tile of it
+  long long item_first;     // first unit of that item
+};
+
+// Sum over the CTA (NT threads, a multiple of 32) of one value a thread, and the sum before it.
+template <int NT>
+VVLI_DEV long long pa_scan(long long v, long long* part, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += a;
+  }
+  __syncthreads();
+  if (lane == 31) part[warp] = s;
+  __syncthreads();
+  long long before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w == warp) before = total;
+    total += part[w];
+  }
+  return before + s - v;
+}
+
+// Tiles of one kv head of request b over all its blocks; a warp works out requests of many blocks together.
+template <int ROWS, int KT>
+VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
+  PaReq r{0, 0, 0};
+  int nb = 0;
+  if (live) r = pa_request(p, b), nb = pa_blocks<ROWS>(p, r);
+  long long u = 0;
+  if (nb <= 8) {
+    for (int i = 0; i < nb; ++i) {
+      const PaItem it = pa_item<ROWS, KT>(p, r, i);
+      u += it.t1 - it.t0;
+    }
+  }
+  unsigned big = __ballot_sync(0xffffffffu, nb > 8);
+  while (big) {
+    const int src = __ffs(big) - 1;
+    big &= big - 1;
+    PaReq o;
+    o.row0 = 0, o.n = __shfl_sync(0xffffffffu, r.n, src), o.pos0 = __shfl_sync(0xffffffffu, r.pos0, src);
+    const int n = __shfl_sync(0xffffffffu, nb, src);
+    long long s = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+      const PaItem it = pa_item<ROWS, KT>(p, o, i);
+      s += it.t1 - it.t0;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if ((threadIdx.x & 31) == src) u = s;
+  }
+  return u;
+}
+
+// This CTA's share, worked out by all its NT threads; valid in `out` (shared) after the call.
+template <int ROWS, int KT, int NT>
+VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, long long* part) {
+  const int tid = threadIdx.x;
+  long long total = 0, t, first_units = 0, first_before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += NT) {
+    const int b = b0 + tid;
+    const long long u = pa_units<ROWS, KT>(p, b, b < p.B) * p.hk;
+    const long long before = pa_scan<NT>(u, part, t);
+    if (b0 == 0) first_units = u, first_before = before;
+    total += t;
+  }
+  const long long grid = gridDim.x;
+  const int active = static_cast<int>(min(grid, total));
+  const long long i = blockIdx.x;
+  const long long u0 = i < active ? total * i / active : 0, u1 = i < active ? total * (i + 1) / active : 0;
+  if (tid == 0) {
+    out->total = total, out->active = active, out->u0 = u0, out->u1 = u1;
+    out->b = p.B;
+  }
+  __syncthreads();
+  long long done = 0;
+  for (int b0 = 0; b0 < p.B && u0 < u1; b0 += NT) {
+    const int b = b0 + tid;
+    long long u = first_units, before = first_before;
+    if (p.B > NT) {  // more requests than threads: the sums again
+      u = pa_units<ROWS, KT>(p, b, b < p.B) * p.hk;
+      before = pa_scan<NT>(u, part, t);
+    } else {
+      t = total;
+    }
+    before += done;
+    if (u > 0 && before <= u0 && u0 < before + u) {
+      const long long per = u / p.hk;
+      out->b = b;
+      out->h = static_cast<int>((u0 - before) / per);
+      out->item_first = before + out->h * per;  // first unit of the head, for now
+    }
+    done += t;
+    if (done > u0) break;  // uniform
+  }
+  __syncthreads();
+  if (tid < 32 && u0 < u1) {  // the block of the head and the tile of the block
+    const PaReq r = pa_request(p, out->b);
+    const int nb = pa_blocks<ROWS>(p, r);
+    long long at = out->item_first;
+    for (int k0 = 0; k0 < nb; k0 += 32) {
+      const int k = k0 + tid;
+      int n = 0;
+      if (k < nb) {
+        const PaItem it = pa_item<ROWS, KT>(p, r, k);
+        n = it.t1 - it.t0;
+      }
+      long long s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, s, o);
+        if (tid >= o) s += a;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, at + s > u0 && at + s - n <= u0 && n > 0);
+      if (hit) {
+        if (tid == __ffs(hit) - 1) out->blk = k, out->item_first = at + s - n, out->off = static_cast<int>(u0 - (at + s - n));
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  __syncthreads();
+}
+
+// A run of tiles of one item.
+struct PaSeg {
+  int b, h, blk;
+  PaReq r;
+  PaItem it;
+  int t0, t1;        // tiles of this segment
+  bool starts, ends;  // the item's first / last tile among them
+  bool at_start;     // the CTA's first segment
+  long long item_first;
+};
+
+template <int ROWS, int KT>
+struct PaWalk {
+  long long u, u1, item_first;
+  int b, h, blk, off;
+  bool first;
+  VVLI_DEV explicit PaWalk(const PaShare& s)
+      : u(s.u0), u1(s.u1), item_first(s.item_first), b(s.b), h(s.h), blk(s.blk), off(s.off), first(true) {}
+  VVLI_DEV bool next(const PaParams& p, PaSeg& s) {
+    if (u >= u1) return false;
+    s.r = pa_request(p, b);
+    while (s.r.n <= 0) s.r = pa_request(p, ++b);  // some later request has the unit u
+    s.b = b, s.h = h, s.blk = blk;
+    s.it = pa_item<ROWS, KT>(p, s.r, blk);
+    s.item_first = item_first;
+    s.at_start = first;
+    s.starts = off == 0;
+    const int left = s.it.t1 - s.it.t0 - off;
+    const int n = static_cast<int>(min(static_cast<long long>(left), u1 - u));
+    s.t0 = s.it.t0 + off;
+    s.t1 = s.t0 + n;
+    s.ends = n == left;
+    first = false;
+    u += n;
+    if (s.ends) {
+      item_first += s.it.t1 - s.it.t0;
+      off = 0;
+      if (++blk >= pa_blocks<ROWS>(p, s.r)) {
+        blk = 0;
+        if (++h >= p.hk) h = 0, ++b;
+      }
+    } else {
+      off += n;
+    }
+    return true;
+  }
+};
+
+// Workspace slot of a segment that is not a whole item.
+VVLI_DEV int pa_slot(const PaSeg& s) { return s.at_start ? 0 : 1; }
+
+// Called by one thread per CTA: what the combine kernel does for it.
+VVLI_DEV void pa_describe(const PaParams& p, const PaShare& sh, const PaSeg* first) {
+  PaDesc d;
+  d.finish = first && !first->starts && first->ends;
+  d.b = d.finish ? first->b : 0, d.h = d.finish ? first->h : 0, d.blk = d.finish ? first->blk : 0;
+  d.item_first = d.finish ? first->item_first : 0;
+  d.active = sh.active, d.total = sh.total, d.pad = 0;
+  p.desc[blockIdx.x] = d;
+}
+
+// ---------------------------------------------------------------- scores
+// In log2 units, so that exp is one ex2: x = s * scale * log2(e), or with a
+// softcap cap * log2(e) * tanh(s * scale / cap), tanh(y) = 1 - 2 / (1 + e^2y)
+// (absolute error below 2^-22, where tanh.approx has 2^-11: a capped score of
+// 50 would be off by 0.02).
+VVLI_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+VVLI_DEV float pa_capped(float s, const PaParams& p) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * p.cap_in)));
+  return p.cap_log2 * fmaf(-2.0f, r, 1.0f);
+}
+
+template <class T>
+VVLI_DEV uint32_t pa_pack(float a, float b);
+template <>
+VVLI_DEV uint32_t pa_pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+VVLI_DEV uint32_t pa_pack<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// TMA load of a box of the cache's 4-D map {64 elements, rows of a page, 64-element slices, pages}.
+VVLI_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The table entry of page pg of request b, or one past the cache (which a TMA load fills with zeros).
+VVLI_DEV int pa_page(const PaParams& p, int b, int pg) {
+  int id = -1;
+  if (pg < p.width) id = __ldg(p.table + static_cast<size_t>(b) * p.width + pg);
+  return id >= 0 && id < p.pages ? id : p.pages;
+}
+
+// ---------------------------------------------------------------- host
+cudaError_t pa_tensor_map(CUtensorMap* map, const void* cache, const vvli_paged_attn_args& a, uint32_t box_rows,
+                          uint32_t box_slices);
+template <class T, int D, int ROWS>
+cudaError_t pa_queue_combine(const PaParams& p, int ctas, cudaStream_t s);
+
+}  // namespace vvli

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const vvli_pag
   const int nt = gridDim.x * kPlanThreads, gt = blockIdx.x * kPlanThreads + tid;
   PlanShared s{plan_smem, plan_smem + B, plan_smem + 2 * B, plan_smem + 3 * B};
   const long long cap = static_cast<long long>(p.max_tokens), width = static_cast<long long>(p.table_width);
-  const long long free0 = min(max(0LL, static_cast<long long>(*p.free_count)), static_cast<long long>(p.pages));
+  const long long free0 = min(max(0LL, static_cast<long long>(*p.free_count)), static_cast<long long>(p.free_entries));
   long long rows = 0, lacking = 0, taken = 0;  // sums over the requests before this chunk
   const bool writer = blockIdx.x == 0;
   // what the writer CTA writes per request once every CTA has read its inputs
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const vvli_pag
         const long long page = at >> shift;
         const int id = page < own ? p.block_table[static_cast<size_t>(b) * p.table_width + page]
                                   : p.free_pages[free0 - 1 - (s.first_page[b] + (page - own))];
-        if (id >= 0 && static_cast<uint64_t>(id) < p.pages) slot = (id << shift) + static_cast<int>(at & (P - 1));
+        if (id >= 0 && id <= (INT_MAX - (P - 1)) >> shift) slot = (id << shift) + static_cast<int>(at & (P - 1));
       }
     }
     p.positions[t] = pos;
@@ -166,8 +166,7 @@ std::string check_plan(const vvli_paged_plan_args* a) {
     return "requests must be in [1, " + std::to_string(kPlanMaxRequests) + "]";
   const std::string page = check_page_size(a->page_size);
   if (!page.empty()) return page;
-  if (a->pages < 1 || a->pages > static_cast<uint64_t>(INT_MAX) / a->page_size)
-    return "pages must be at least 1 with pages * page_size < 2^31";
+  if (a->free_entries < 1 || a->free_entries > INT_MAX) return "free_entries must be in [1, 2^31)";
   if (a->table_width < 1 || a->table_width > INT_MAX) return "table_width must be in [1, 2^31)";
   if (a->max_tokens > INT_MAX) return "max_tokens must be below 2^31";
   const void* need[] = {a->context,    a->new_tokens, a->owned,     a->block_table,    a->free_pages, a->free_count,

@@ -1,5 +1,5 @@
 """Host side of the paged serving step (include/vvli_cuda.h: vvli_cuda_paged_plan,
-vvli_cuda_qk_rope_write).
+vvli_cuda_qk_rope_write, vvli_cuda_paged_attention).
 
 The reference keeps one contiguous fp32 cache per sequence (KVCache,
 src/llm.zig:539-606) and moves one token at a time (src/llm.zig:702-709).
@@ -8,7 +8,10 @@ These operators serve many requests, each with any number of new tokens, over
 
     step = plan_step(context, new, owned, block_table, free_pages, free_count, page_size, rows)
     q = qk_norm_rope_write(q, k, v, k_cache, v_cache, step.slots, step.positions, inv_freq, ...)
+    out = attention(q, k_cache, v_cache, block_table, step.cu_new, step.seq_len, max_new)
 
+with attention = PagedAttention(q_heads, kv_heads, head_dim, page_size), which
+keeps the workspace; vvli_b200.speculative.verify_drafts ends a step of drafts.
 A cache is a [pages][kv heads][page_size][head_dim] tensor (pages may be
 further apart).  Device memory is handled with torch tensors (plumbing only).
 Work is queued on ``stream`` (the current stream of the tensors' device when
@@ -90,7 +93,7 @@ def plan_step(context, new, owned, block_table, free_pages, free_count, page_siz
 
     context, new, owned: int32 [requests], each request's cached tokens, new
     tokens and owned pages; block_table: int32 [requests][width], extended in
-    place; free_pages: int32 [pages], a stack of which the first free_count[0]
+    place; free_pages: int32, a stack of which the first free_count[0]
     entries are free.  max_tokens: rows of the step (a captured step may have
     more than are used).  With inplace=True, owned and free_count are updated
     themselves (and are the plan's)."""
@@ -170,3 +173,77 @@ def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_fre
     if T:
         check(_abi.lib().vvli_cuda_qk_rope_write(dev.index, ctypes.byref(a), _stream(dev, stream)))
     return out
+
+
+class PagedAttention:
+    """Attention of the requests' new tokens over their pages (vvli_cuda_paged_attention).
+
+    Row i of request b (q rows cu_new[b] ..) sees the keys up to its position
+    seq_len[b] - new[b] + i, with ``window`` > 0 only the last ``window`` of them;
+    scores are scale * q.k (1 / sqrt(head_dim) by default), capped by
+    softcap * tanh(s / softcap) when softcap > 0, plus alibi[head] * (key
+    position - query position) when alibi (float32 [q_heads]) is given.  The
+    workspace (its size depends on head_dim alone) is allocated here: calls of
+    one object, and graphs captured from them, must not run at the same time.
+    """
+
+    def __init__(self, q_heads: int, kv_heads: int, head_dim: int, page_size: int, dtype=torch.bfloat16, scale=None,
+                 softcap: float = 0.0, window: int = 0, alibi=None, device: int | torch.device | None = None):
+        if dtype not in _DTYPES:
+            raise ValueError("PagedAttention: dtype must be bf16 or fp16")
+        need = int(_abi.lib().vvli_cuda_paged_attn_workspace_bytes(max(0, int(head_dim))))
+        if need == 0:
+            raise ValueError("PagedAttention: head_dim must be 64 or 128")
+        if device is None:
+            device = torch.cuda.current_device()
+        self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if alibi is not None and (alibi.dtype != torch.float32 or alibi.numel() != q_heads or not alibi.is_contiguous()
+                                  or alibi.device != self.device):
+            raise ValueError(f"PagedAttention: alibi must be {q_heads} contiguous float32 values on {self.device}")
+        self.q_heads, self.kv_heads, self.head_dim, self.page_size = q_heads, kv_heads, head_dim, page_size
+        self.dtype, self.alibi = dtype, alibi
+        self.scale = float(head_dim) ** -0.5 if scale is None else float(scale)
+        self.softcap, self.window = float(softcap), int(window)
+        if self.window < 0:
+            raise ValueError("PagedAttention: window must be >= 0")
+        self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self._ws[:4].zero_()
+
+    def __call__(self, q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: int, out=None, lse=False, stream=None):
+        """q: [rows][q_heads][head_dim]; block_table: int32 [requests][width]; cu_new: int32 [requests + 1] and seq_len:
+        int32 [requests], as plan_step gives them; max_new: the longest request's new tokens (picks the kernel).
+        Returns out ([rows][q_heads][head_dim], new unless given; rows of no request are not written), and with
+        lse=True, or a float32 [rows][q_heads] tensor for it, (out, lse)."""
+        who, dev, dtype = "PagedAttention", self.device, self.dtype
+        qs = _heads(who, "q", q, dtype, dev)
+        T, hq, d = q.shape
+        if hq != self.q_heads or d != self.head_dim:
+            raise ValueError(f"PagedAttention: q must be [rows][{self.q_heads}][{self.head_dim}]")
+        pages, page_size, page_stride = _cache_layout(who, k_cache, v_cache, self.kv_heads, d, dtype, dev)
+        if page_size != self.page_size:
+            raise ValueError(f"PagedAttention: the caches' pages must have {self.page_size} positions")
+        B = seq_len.numel()
+        if block_table.dim() != 2 or block_table.shape[0] < B:
+            raise ValueError("PagedAttention: block_table must be [requests][width]")
+        if out is None:
+            out = _empty((T, hq, d), dtype, dev, stream)
+        elif out.shape != q.shape:
+            raise ValueError("PagedAttention: out must have q's shape")
+        if lse is True:
+            lse = _empty((T, hq), torch.float32, dev, stream)
+        elif lse is not False and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (T, hq)
+                                   or not lse.is_contiguous()):
+            raise ValueError(f"PagedAttention: lse must be a contiguous [{T}][{hq}] float32 tensor on {dev}")
+        a = _abi.CPagedAttnArgs(
+            B, T, hq, self.kv_heads, d, page_size, pages, page_stride, block_table.shape[1], qs,
+            _heads(who, "out", out, dtype, dev), max(0, int(max_new)), self.window, _DTYPES[dtype], self.scale, self.softcap, 0,
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+            None if lse is False else lse.data_ptr(), None if self.alibi is None else self.alibi.data_ptr(),
+            _ints(who, "block_table", block_table, dev), _ints(who, "cu_new", cu_new, dev, B + 1),
+            _ints(who, "seq_len", seq_len, dev), self._ws.data_ptr(), self._ws.numel())
+        check(_abi.lib().vvli_cuda_paged_attention(dev.index, ctypes.byref(a), _stream(dev, stream)))
+        return out if lse is False else (out, lse)
+
+    def status(self) -> int:
+        """0, or VVLI_ERR_TIMEOUT (22) once a bounded wait of a call has given up (synchronises)."""
+        return int(self._ws[:4].view(torch.int32).item())
