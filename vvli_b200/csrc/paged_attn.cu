@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2] = {0.f, 0.f};
     float o[D / 8][4];
     {
+      const uint32_t sign = p.negate ? 0x80008000u : 0u;
       const uint16_t* src[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint16_t* a = src[j & 1];
-          qf[ks][j] = a ? *reinterpret_cast<const uint32_t*>(a + 16 * ks + 8 * (j >> 1) + 2 * t4) : 0u;
+          qf[ks][j] = a ? *reinterpret_cast<const uint32_t*>(a + 16 * ks + 8 * (j >> 1) + 2 * t4) ^ sign : 0u;
         }
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -406,12 +407,17 @@ cudaError_t launch_short(int device, const PaParams& p, const vvli_paged_attn_ar
   return pa_queue_combine<T, D, 16 * RG>(p, ctas, s);
 }
 
+// Blocks of 16 or 32 rows while they hold a request's rows; beyond, every block of
+// 32 would stream the request's keys again, and the tensor-core kernel's blocks
+// have 256 rows.
 template <class T, int D>
-cudaError_t short_variant(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
-  const bool feat = p.cap_log2 > 0.f || p.alibi;
-  if (a.max_new * p.G <= 16)
+cudaError_t queue_variant(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
+  const bool feat = pa_featured(p);
+  if (a.max_new <= 16u / p.G)
     return feat ? launch_short<T, D, 1, true>(device, p, a, ctas, s) : launch_short<T, D, 1, false>(device, p, a, ctas, s);
-  return feat ? launch_short<T, D, 2, true>(device, p, a, ctas, s) : launch_short<T, D, 2, false>(device, p, a, ctas, s);
+  if (a.max_new <= 32u / p.G)
+    return feat ? launch_short<T, D, 2, true>(device, p, a, ctas, s) : launch_short<T, D, 2, false>(device, p, a, ctas, s);
+  return pa_queue_tc<T, D>(device, p, a, ctas, s);
 }
 
 std::string check_attn(const vvli_paged_attn_args* a) {
@@ -468,7 +474,8 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.pages = static_cast<int>(a.pages), p.width = static_cast<int>(a.table_width);
   p.window = static_cast<int>(a.window);
   constexpr double kLog2e = 1.44269504088896340736;
-  p.scale_log2 = static_cast<float>(a.scale * kLog2e);
+  p.negate = a.scale < 0.f && !(a.softcap > 0.f) && !a.alibi;
+  p.scale_log2 = static_cast<float>((p.negate ? -a.scale : a.scale) * kLog2e);
   if (a.softcap > 0.f) {
     p.cap_in = static_cast<float>(static_cast<double>(a.scale) / a.softcap * 2.0 * kLog2e);
     p.cap_log2 = static_cast<float>(a.softcap * kLog2e);
@@ -484,10 +491,10 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.part_o = p.part_ml + static_cast<size_t>(kPaMaxCtas) * 2 * kPaMaxRows * 2;
   static_assert((256 + kPaMaxCtas * sizeof(PaDesc)) % 16 == 0, "the parts are 16-byte aligned");
   if (a.dtype == VVLI_BF16)
-    return a.head_dim == 64 ? short_variant<__nv_bfloat16, 64>(device, p, a, ctas, s)
-                            : short_variant<__nv_bfloat16, 128>(device, p, a, ctas, s);
-  return a.head_dim == 64 ? short_variant<__half, 64>(device, p, a, ctas, s)
-                          : short_variant<__half, 128>(device, p, a, ctas, s);
+    return a.head_dim == 64 ? queue_variant<__nv_bfloat16, 64>(device, p, a, ctas, s)
+                            : queue_variant<__nv_bfloat16, 128>(device, p, a, ctas, s);
+  return a.head_dim == 64 ? queue_variant<__half, 64>(device, p, a, ctas, s)
+                          : queue_variant<__half, 128>(device, p, a, ctas, s);
 }
 
 }  // namespace
@@ -529,6 +536,11 @@ cudaError_t pa_tensor_map(CUtensorMap* map, const void* cache, const vvli_paged_
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
+
+template cudaError_t pa_queue_combine<__nv_bfloat16, 64, kPaMaxRows>(const PaParams&, int, cudaStream_t);
+template cudaError_t pa_queue_combine<__nv_bfloat16, 128, kPaMaxRows>(const PaParams&, int, cudaStream_t);
+template cudaError_t pa_queue_combine<__half, 64, kPaMaxRows>(const PaParams&, int, cudaStream_t);
+template cudaError_t pa_queue_combine<__half, 128, kPaMaxRows>(const PaParams&, int, cudaStream_t);
 
 }  // namespace vvli
 

@@ -41,7 +41,8 @@ struct PaDesc {  // what the combine kernel needs of a CTA
 struct PaParams {
   int B, T, hq, hk, G, shift, pages, width;  // page_size = 1 << shift
   int window;                                // 0: none
-  float scale_log2;                          // scale * log2(e)
+  float scale_log2;                          // scale * log2(e); its magnitude without a feature, then
+  int negate;                                // the sign goes into q
   float cap_in, cap_log2;                    // softcap: scale / cap * 2 log2(e); cap * log2(e); 0 without
   long long q_stride, out_stride;
   const uint16_t* q;
@@ -60,6 +61,9 @@ inline size_t pa_workspace_bytes(int d) {
   const size_t slots = static_cast<size_t>(kPaMaxCtas) * 2 * kPaMaxRows;
   return 256 + kPaMaxCtas * sizeof(PaDesc) + slots * 2 * sizeof(float) + slots * d * sizeof(float);
 }
+
+// Softcap, ALiBi, or a scale too small to be undone: the kernels' general score path.
+inline bool pa_featured(const PaParams& p) { return p.cap_log2 > 0.f || p.alibi || !(p.scale_log2 > 1e-30f); }
 
 // ---------------------------------------------------------------- schedule
 
@@ -343,6 +347,9 @@ VVLI_DEV int pa_page(const PaParams& p, int b, int pg) {
 // ---------------------------------------------------------------- host
 cudaError_t pa_tensor_map(CUtensorMap* map, const void* cache, const vvli_paged_attn_args& a, uint32_t box_rows,
                           uint32_t box_slices);
+// The tensor-core kernel (paged_attn_tc.cu) and, for either, the combine kernel (paged_attn.cu).
+template <class T, int D>
+cudaError_t pa_queue_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s);
 template <class T, int D, int ROWS>
 cudaError_t pa_queue_combine(const PaParams& p, int ctas, cudaStream_t s);
 
