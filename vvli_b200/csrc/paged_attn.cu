@@ -412,7 +412,7 @@ cudaError_t launch_short(int device, const PaParams& p, const vvli_paged_attn_ar
 // have 256 rows.
 template <class T, int D>
 cudaError_t queue_variant(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
-  const bool feat = pa_featured(p);
+  const bool feat = pa_features(p) != 0;
   if (a.max_new <= 16u / p.G)
     return feat ? launch_short<T, D, 1, true>(device, p, a, ctas, s) : launch_short<T, D, 1, false>(device, p, a, ctas, s);
   if (a.max_new <= 32u / p.G)
@@ -477,6 +477,7 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.negate = a.scale < 0.f && !(a.softcap > 0.f) && !a.alibi;
   p.scale_log2 = static_cast<float>((p.negate ? -a.scale : a.scale) * kLog2e);
   if (a.softcap > 0.f) {
+    p.cap_y = a.scale / a.softcap;
     p.cap_in = static_cast<float>(static_cast<double>(a.scale) / a.softcap * 2.0 * kLog2e);
     p.cap_log2 = static_cast<float>(a.softcap * kLog2e);
   }

@@ -43,7 +43,7 @@ struct PaParams {
   int window;                                // 0: none
   float scale_log2;                          // scale * log2(e); its magnitude without a feature, then
   int negate;                                // the sign goes into q
-  float cap_in, cap_log2;                    // softcap: scale / cap * 2 log2(e); cap * log2(e); 0 without
+  float cap_y, cap_in, cap_log2;             // softcap: scale / cap; that times 2 log2(e); cap * log2(e), 0 without
   long long q_stride, out_stride;
   const uint16_t* q;
   uint16_t* out;
@@ -62,8 +62,13 @@ inline size_t pa_workspace_bytes(int d) {
   return 256 + kPaMaxCtas * sizeof(PaDesc) + slots * 2 * sizeof(float) + slots * d * sizeof(float);
 }
 
-// Softcap, ALiBi, or a scale too small to be undone: the kernels' general score path.
-inline bool pa_featured(const PaParams& p) { return p.cap_log2 > 0.f || p.alibi || !(p.scale_log2 > 1e-30f); }
+// Variants of the score arithmetic.  Without either, exp's argument is one FMA
+// of the raw score; a scale too small for that (0 among them) takes the ALiBi
+// form, with slopes of 0.
+enum : int { kPaCap = 1, kPaAlibi = 2 };
+inline int pa_features(const PaParams& p) {
+  return p.cap_log2 > 0.f ? kPaCap | (p.alibi ? kPaAlibi : 0) : p.alibi || !(p.scale_log2 > 1e-30f) ? kPaAlibi : 0;
+}
 
 // ---------------------------------------------------------------- schedule
 

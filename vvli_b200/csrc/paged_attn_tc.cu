@@ -46,7 +46,7 @@ struct TcaLayout {
   static constexpr uint32_t stages = 131072 / kv;      // 4 at D 128, 8 at D 64; keys and values in turn
   static constexpr uint32_t ring = 2 * q_tile;
   static constexpr uint32_t bars = ring + stages * kv;
-  static constexpr uint32_t share = bars + 320;        // 3 stages + 9 barriers and the TMEM address
+  static constexpr uint32_t share = bars + 320;        // 3 stages + 11 barriers and the TMEM address
   static constexpr uint32_t part = share + 64;
   static constexpr uint32_t smem = part + 128 + 1024;  // + alignment slack
   static constexpr uint32_t o_col = 256;               // S_0 at column 0, S_1 at 128, O_t at 256 + D t
@@ -71,12 +71,28 @@ constexpr uint32_t tca_idesc(int N, bool b_mn) {
   return (1u << 4) | (type << 7) | (type << 10) | (b_mn ? 1u << 16 : 0u) | ((static_cast<uint32_t>(N) >> 3) << 17) |
          ((128u >> 4) << 24);
 }
-// D += A B with A in TMEM (rows = lanes, two 16-bit elements a column).
-VVLI_DEV void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The MMA warp runs as one (so that ptxas keeps addresses and descriptors in
+// uniform registers: with one thread branched off, an MMA took about 90 cycles
+// to issue and 64 to run), and one elected lane issues.
+VVLI_DEV void tca_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D += A B with A in TMEM (rows = lanes, two 16-bit elements a column).
+VVLI_DEV void tca_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+VVLI_DEV void tca_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
 
@@ -115,6 +131,76 @@ VVLI_DEV void tca_st32(uint32_t taddr, const uint32_t* v) {
 VVLI_DEV void tca_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 VVLI_DEV void tca_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Pairs of fp32 operations in one instruction.
+VVLI_DEV uint64_t f2_bits(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+VVLI_DEV float2 f2_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+VVLI_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_of(r);
+}
+VVLI_DEV float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+VVLI_DEV float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+VVLI_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The capped scores of a row, in log2 units.  tanh by its formula takes two
+// exponential-unit operations a score beside the softmax's one, on the unit
+// that bounds this kernel; scores are mostly well below the cap, and there
+// tanh(y) = y P(y^2) on the FMA units: P is the degree-5 minimax fit of
+// tanh(y) / y on y^2 <= 0.75^2, found by iterated reweighted least squares
+// (relative error below 3e-8).  One branch per warp and tile.
+VVLI_DEV void tca_cap(const PaParams& p, float* s) {
+  float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 128; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) big[k] = max3(big[k], fabsf(s[i + 2 * k]), fabsf(s[i + 2 * k + 1]));
+  const float y = max3(fmaxf(big[0], big[1]), big[2], big[3]) * fabsf(p.cap_y);
+  if (__any_sync(0xffffffffu, !(y <= 0.75f))) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i) s[i] = pa_capped(s[i], p);
+    return;
+  }
+  const float2 in = make_float2(p.cap_y, p.cap_y);
+  const float c = p.cap_log2;
+  const float2 c0 = make_float2(c * 0.9999999710138239f, c * 0.9999999710138239f);
+  const float2 c1 = make_float2(c * -0.3333295887885829f, c * -0.3333295887885829f);
+  const float2 c2 = make_float2(c * 0.13325406008965843f, c * 0.13325406008965843f);
+  const float2 c3 = make_float2(c * -0.05334442971164088f, c * -0.05334442971164088f);
+  const float2 c4 = make_float2(c * 0.019582907313611682f, c * 0.019582907313611682f);
+  const float2 c5 = make_float2(c * -0.004716256631635093f, c * -0.004716256631635093f);
+#pragma unroll
+  for (int i = 0; i < 128; i += 2) {
+    const float2 v = mul2(make_float2(s[i], s[i + 1]), in), u = mul2(v, v);
+    float2 r = fma2(c5, u, c4);
+    r = fma2(r, u, c3);
+    r = fma2(r, u, c2);
+    r = fma2(r, u, c1);
+    r = mul2(fma2(r, u, c0), v);
+    s[i] = r.x, s[i + 1] = r.y;
+  }
+}
+
 // Tiles of this segment that row tile t works on (its rows see no later key).
 VVLI_DEV int tca_tiles(const PaParams& p, const PaSeg& s, int t) {
   const int rows = min(kTcTile, s.it.rows - t * kTcTile);
@@ -124,7 +210,7 @@ VVLI_DEV int tca_tiles(const PaParams& p, const PaSeg& s, int t) {
   return max(0, min(s.t1, end) - s.t0);
 }
 
-template <class T, int D, bool FEAT>
+template <class T, int D, int FEAT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using L = TcaLayout<D>;
@@ -138,10 +224,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* v_ready = empty + ST;                              // [ST] a stage's values, cleared where nothing is seen
   uint64_t* q_full = v_ready + ST;                             // [2] Q_t is in shared memory
   uint64_t* s_full = q_full + 2;                               // [2] S_t is in TMEM (and the P V before it done)
-  uint64_t* p_full = q_full + 4;                               // [2] P_t is in TMEM (and O_t rescaled)
-  uint64_t* o_full = q_full + 6;                               // [2] the segment's last P_t V is done
-  uint64_t* drained = q_full + 8;                              // every MMA is done
-  uint32_t* holder = reinterpret_cast<uint32_t*>(q_full + 9);
+  uint64_t* p_half = q_full + 4;                               // [2] P_t of the first 64 keys is in TMEM (and O_t rescaled)
+  uint64_t* p_full = q_full + 6;                               // [2] all of P_t is
+  uint64_t* o_full = q_full + 8;                               // [2] the segment's last P_t V is done
+  uint64_t* drained = q_full + 10;                             // every MMA is done
+  uint32_t* holder = reinterpret_cast<uint32_t*>(q_full + 11);
   PaShare* share = reinterpret_cast<PaShare*>(sm + L::share);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -150,7 +237,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int s = 0; s < ST; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&v_ready[s], 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], kTcTile), mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], kTcTile), mbar_init(&o_full[t], 1);
+      mbar_init(&p_half[t], kTcTile), mbar_init(&p_full[t], kTcTile), mbar_init(&o_full[t], 1);
     }
     mbar_init(drained, 1);
     fence_barrier_init();
@@ -168,9 +255,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   PaSeg sg;
   bool dead = false;  // a wait gave up: the rest is skipped
 
-  // The register file's 384 x 168 are split anew: 256 x 208 for the softmax, 128 x 88 for the rest.
+  // The register file's 384 x 168 are split anew: 256 x 200 for the softmax, 128 x 104 for the rest.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 9) {  // ---- copies
       int n = 0;      // copies into the ring so far
       const int rows_page = 1 << p.shift;
@@ -230,72 +317,78 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) mbar_arrive(&v_ready[s]);
         }
       }
-    } else if (warp == 8) {  // ---- MMAs, by one thread
-      if (lane == 0) {
-        constexpr uint32_t s_idesc = tca_idesc<T>(kTcKeys, false), o_idesc = tca_idesc<T>(D, true);
-        const uint64_t dq = umma_desc(base), dk = umma_desc(base + L::ring), dv = tca_mn_desc(base + L::ring);
-        int n = 0;                                // stages used before this segment
-        uint32_t qs[2] = {0, 0}, ps[2] = {0, 0};  // waits on q_full, p_full so far
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-          if (!dead) dead = !mbar_wait(bar, parity & 1, p.err);
-          tc_fence_after();
-        };
-        while (!dead && walk.next(p, sg)) {
-          const int N = sg.t1 - sg.t0;
-          const int nt[2] = {tca_tiles(p, sg, 0), tca_tiles(p, sg, 1)};
-          auto issue_s = [&](int t, int j) {
-            const int s = (n + 2 * j) % ST;
-            const uint64_t a = dq + ((t * L::q_tile) >> 4), b = dk + ((s * L::kv) >> 4);
+    } else if (warp == 8) {  // ---- MMAs
+      constexpr uint32_t s_idesc = tca_idesc<T>(kTcKeys, false), o_idesc = tca_idesc<T>(D, true);
+      const uint64_t dq = umma_desc(base), dk = umma_desc(base + L::ring), dv = tca_mn_desc(base + L::ring);
+      uint32_t n = 0;                                          // stages used before this segment
+      uint32_t q_par0 = 0, q_par1 = 0, p_par0 = 0, p_par1 = 0;  // parities of the next waits on q_full, p_half / p_full
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity & 1)) && !dead)
+          dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
+      };
+      auto issue_s = [&](int t, uint32_t stage) {
+        const uint64_t a = dq + ((t * L::q_tile) >> 4), b = dk + stage * (L::kv >> 4);
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t o = ((ks >> 2) * L::slice + (ks & 3) * 32) >> 4;
-              umma_bf16(tmem + t * 128, a + o, b + o, s_idesc, ks != 0);
-            }
-            umma_commit(&s_full[t]);
-          };
-          auto issue_pv = [&](int t, int j) {
-            const int s = (n + 2 * j + 1) % ST;
-            const uint64_t b = dv + ((s * L::kv) >> 4);
-#pragma unroll
-            for (int ks = 0; ks < kTcKeys / 16; ++ks)
-              umma_ts(tmem + L::o_col + t * D, tmem + t * 128 + ks * 8, b + ((ks * 16 * 128) >> 4), o_idesc, (j | ks) != 0);
-          };
-          wait(&full[n % ST], n / ST);
-          for (int t = 0; t < 2; ++t) {
-            if (nt[t] == 0) continue;
-            wait(&q_full[t], qs[t]++);
-            if (!dead) issue_s(t, 0);
-          }
-          if (!dead) umma_commit(&empty[n % ST]);
-          for (int j = 0; j < N && !dead; ++j) {
-            const int vs = n + 2 * j + 1, ks = vs + 1;
-            const bool next = j + 1 < N;
-            wait(&v_ready[vs % ST], vs / ST);
-            bool k_in = false;
-            for (int t = 0; t < 2; ++t) {
-              if (j < nt[t]) {
-                wait(&p_full[t], ps[t]++);
-                if (!dead) issue_pv(t, j);
-                if (!dead && j + 1 == nt[t]) umma_commit(&o_full[t]);
-              }
-              if (j + 1 < nt[t]) {
-                if (!k_in) wait(&full[ks % ST], ks / ST), k_in = true;
-                if (!dead) issue_s(t, j + 1);
-              }
-            }
-            if (!dead) umma_commit(&empty[vs % ST]);
-            if (next && !k_in) wait(&full[ks % ST], ks / ST);
-            if (next && !dead) umma_commit(&empty[ks % ST]);
-          }
-          n += 2 * N;
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t o = ((ks >> 2) * L::slice + (ks & 3) * 32) >> 4;
+          tca_mma(tmem + t * 128, a + o, b + o, s_idesc, ks != 0);
         }
-        umma_commit(drained);
-        mbar_wait(drained, 0, p.err);
+        tca_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int t, uint32_t stage, int half, uint32_t more) {  // 64 of the tile's keys
+        const uint64_t b = dv + stage * (L::kv >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int ks = 4 * half + i;
+          tca_mma_ts(tmem + L::o_col + t * D, tmem + t * 128 + ks * 8, b + ((ks * 16 * 128) >> 4), o_idesc, more | ks);
+        }
+      };
+      // P V of tile j and S of tile j + 1
+      auto step = [&](int t, int j, int nt, uint32_t& par, uint32_t vs, uint32_t ks) {
+        if (j < nt) {
+          wait(&p_half[t], par);
+          tc_fence_after();
+          if (!dead) issue_pv(t, vs, 0, j);
+          wait(&p_full[t], par);
+          tc_fence_after();
+          par ^= 1;
+          if (!dead) issue_pv(t, vs, 1, j);
+          if (!dead && j + 1 == nt) tca_commit(&o_full[t]);
+        }
+        if (!dead && j + 1 < nt) issue_s(t, ks);
+      };
+      while (!dead && walk.next(p, sg)) {
+        const int N = sg.t1 - sg.t0, nt0 = tca_tiles(p, sg, 0), nt1 = tca_tiles(p, sg, 1);
+        wait(&full[n % ST], n / ST);
+        if (nt0) {
+          wait(&q_full[0], q_par0);
+          q_par0 ^= 1;
+          if (!dead) issue_s(0, n % ST);
+        }
+        if (nt1) {
+          wait(&q_full[1], q_par1);
+          q_par1 ^= 1;
+          if (!dead) issue_s(1, n % ST);
+        }
+        if (!dead) tca_commit(&empty[n % ST]);
+        for (int j = 0; j < N && !dead; ++j) {
+          const uint32_t v = n + 2 * j + 1, k = v + 1;
+          wait(&v_ready[v % ST], v / ST);
+          if (j + 1 < N) wait(&full[k % ST], k / ST);
+          step(0, j, nt0, p_par0, v % ST, k % ST);
+          step(1, j, nt1, p_par1, v % ST, k % ST);
+          if (dead) break;
+          tca_commit(&empty[v % ST]);
+          if (j + 1 < N) tca_commit(&empty[k % ST]);
+        }
+        n += 2 * N;
       }
+      tca_commit(drained);
+      mbar_wait(drained, 0, p.err);
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax of row tile t: thread = row
     const int t = warp >> 2, R = kTcTile * t + 32 * (warp & 3) + lane;  // row of the item
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
@@ -314,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int first_pos = sg.r.pos0 + (sg.blk * kTcRows + t * kTcTile) / p.G;  // of this tile's first row
       const int last_pos = sg.it.hi - 1;
       float m = -INFINITY, l = 0.f;
-      const float slope = FEAT && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
+      const float slope = (FEAT & kPaAlibi) && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
       if (nt > 0) {
         const uint16_t* src = p.q + (sg.r.row0 + tok) * p.q_stride + static_cast<long long>(head) * D;
         uint4 v[D / 8];
@@ -341,11 +434,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) tca_pin(s + 32 * c);
         const int key0 = (sg.t0 + j) * kTcKeys;
         const int lim = pos - key0;  // columns up to here are visible
-        if constexpr (FEAT) {
+        if constexpr (FEAT & kPaCap) tca_cap(p, s);
+        if constexpr (FEAT & kPaAlibi) {
+          const float2 sl = make_float2(slope, slope), at = make_float2(-static_cast<float>(lim), -static_cast<float>(lim));
+          const float2 unit2 = make_float2(p.scale_log2, p.scale_log2);
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            const float x = p.cap_log2 > 0.f ? pa_capped(s[i], p) : s[i] * p.scale_log2;
-            s[i] = fmaf(slope, static_cast<float>(i - lim), x);
+          for (int i = 0; i < 128; i += 2) {
+            const float2 d = add2(make_float2(i, i + 1), at);  // key - query position, exact below 2^24
+            float2 x = make_float2(s[i], s[i + 1]);
+            if constexpr (!(FEAT & kPaCap)) x = mul2(x, unit2);
+            x = fma2(sl, d, x);
+            s[i] = x.x, s[i + 1] = x.y;
           }
         }
         if (key0 + kTcKeys - 1 > first_pos || (p.window && key0 <= last_pos - p.window)) {  // uniform over the warp
@@ -355,9 +454,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
         const float unit = FEAT ? 1.0f : p.scale_log2;  // s * unit is in log2 units; > 0
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * unit;
+        const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * unit;
         const bool rise = mt > m + kTcRise;  // m = -inf: any finite mt
         if (__any_sync(0xffffffffu, rise)) {
           const float alpha = rise ? ex2(m - mt) : 1.0f;  // m = -inf: 0
@@ -378,29 +481,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         const float mu = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 unit2 = make_float2(unit, unit), low2 = make_float2(-mu, -mu);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t w[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float a = ex2(fmaf(s[64 * h + 2 * i], unit, -mu)), b = ex2(fmaf(s[64 * h + 2 * i + 1], unit, -mu));
-            sum[(2 * i) & 3] += a, sum[(2 * i + 1) & 3] += b;
-            w[i] = pa_pack<T>(a, b);
+            float2 x = fma2(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), unit2, low2);
+            x.x = ex2(x.x), x.y = ex2(x.y);
+            sum[i & 1] = add2(sum[i & 1], x);
+            w[i] = pa_pack<T>(x.x, x.y);
           }
           tca_st32(ts + 32 * h, w);
+          tca_st_done();
+          tc_fence_before();
+          mbar_arrive(h == 0 ? &p_half[t] : &p_full[t]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tca_st_done();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
       }
       if (dead) break;
       if (nt > 0) wait(&o_full[t], os++);
       if (dead) break;
       const bool whole = sg.starts && sg.ends;
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
-      const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);
+      const float inv = m == -INFINITY && l == l ? 0.f : 1.0f / l;  // no visible key: zeros; NaN stays
       if (live) {
         if (whole) {
           if (p.lse)
@@ -443,7 +549,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-template <class T, int D, bool FEAT>
+template <class T, int D, int FEAT>
 cudaError_t launch_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
   static std::once_flag once[kOpMaxDevices];
   static cudaError_t ready[kOpMaxDevices];
@@ -465,7 +571,12 @@ cudaError_t launch_tc(int device, const PaParams& p, const vvli_paged_attn_args&
 
 template <class T, int D>
 cudaError_t pa_queue_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
-  return pa_featured(p) ? launch_tc<T, D, true>(device, p, a, ctas, s) : launch_tc<T, D, false>(device, p, a, ctas, s);
+  switch (pa_features(p)) {
+    case 0: return launch_tc<T, D, 0>(device, p, a, ctas, s);
+    case kPaCap: return launch_tc<T, D, kPaCap>(device, p, a, ctas, s);
+    case kPaAlibi: return launch_tc<T, D, kPaAlibi>(device, p, a, ctas, s);
+    default: return launch_tc<T, D, kPaCap | kPaAlibi>(device, p, a, ctas, s);
+  }
 }
 template cudaError_t pa_queue_tc<__nv_bfloat16, 64>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
 template cudaError_t pa_queue_tc<__nv_bfloat16, 128>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
