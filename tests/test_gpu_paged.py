@@ -263,3 +263,10 @@ def test_plan_and_write_captured_on_another_stream(torch):
         if s >= 0:
             assert torch.equal(caches[0][s // page, :, s % page], k[t])
     assert int((caches[1] != 0).any(-1).sum()) == 2 * sum(s >= 0 for s in want[3])
+
+
+def test_qk_row_norm_in_place_over_many_heads(torch):
+    # more heads than one pass of a CTA takes: every head is read for the row's norm before any is overwritten
+    inp = make_qk(torch, 11, 21, 96, 24, 128, 32, torch.bfloat16, "row", 64)
+    for _ in range(3):
+        check_qk(torch, inp, "row", False, inplace=True)

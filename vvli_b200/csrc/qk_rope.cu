@@ -24,7 +24,7 @@ using namespace vvli;
 
 namespace {
 
-constexpr int kQkThreads = 256;
+constexpr int kQkMaxThreads = 256;
 constexpr int kQkMaxTokens = 8;  // tokens of a CTA
 
 template <class T>
@@ -66,10 +66,9 @@ VVLI_DEV void st16(void* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; 
 struct QkDev {
   int tokens, hq, hk, d, pairs, shift;  // page_size = 1 << shift
   int per_cta;                          // tokens of a CTA
-  int interleaved;
   unsigned slots_end;                   // pages << shift
   long long page_stride, q_stride, k_stride, v_stride, out_stride;
-  float eps;
+  float eps, q_share, k_share;  // 1 over the values of a mean
   const uint16_t *q, *k, *v;
   uint16_t *q_out, *k_cache, *v_cache;
   const uint16_t *q_weight, *k_weight;
@@ -77,128 +76,135 @@ struct QkDev {
   const double* inv_freq;
 };
 
-// NORM: enum vvli_qk_norm.  LANES: threads of a head, head_dim / 16 rounded up
-// to a power of two (LANES <= 16, so a head stays in a warp).
-template <class T, int NORM, int LANES>
-__global__ void __launch_bounds__(kQkThreads) qk_rope_kernel(const QkDev p) {
-  extern __shared__ float2 turn[];  // [tokens of the CTA][pairs] cosine, sine
-  __shared__ float row_sum[2][kQkMaxTokens][kQkThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// PAIRED: interleaved pairs.  NORM: enum vvli_qk_norm.  LANES: threads of a
+// head, head_dim / 16 rounded up to a power of two (LANES <= 16, so a head stays
+// in a warp).  CTA (x, y): tokens x * per_cta .. and part y of the heads;
+// a thread keeps its head and chunks, hence its weights, for all tokens.
+template <class T, int NORM, int LANES, bool PAIRED>
+__global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p) {
+  extern __shared__ __align__(16) float2 turn[];  // [tokens of the CTA][pairs] cosine, sine
+  __shared__ float row_sum[2][kQkMaxTokens][kQkMaxThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int t0 = blockIdx.x * p.per_cta, nt = min(p.per_cta, p.tokens - t0);
-  const int j = tid % LANES;  // chunk pair within the head
-  const int heads = p.hq + 2 * p.hk, chunks = p.d >> 4;
-  const int c0 = !p.interleaved && 8 * j < p.pairs ? j : 2 * j;
-  // chunk c's partner; the part past 2 * pairs starts at an even chunk
-  const int c1 = !p.interleaved && 8 * j < p.pairs ? j + (p.pairs >> 3) : 2 * j + 1;
+  const int j = tid % LANES, chunks = p.d >> 4;  // chunk pair within the head
   const bool turned = 8 * j < p.pairs;
-
-  for (int i = tid; i < nt * p.pairs; i += kQkThreads) {
-    const int t = i / p.pairs, f = i - t * p.pairs;
-    constexpr double kInvTwoPi = 0.15915494309189533576888;
-    const double turns = static_cast<double>(p.positions[t0 + t]) * p.inv_freq[f] * kInvTwoPi;
-    float s, c;
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-    turn[i] = make_float2(c, s);
-  }
-  if constexpr (NORM == VVLI_NORM_ROW) {
-    // mean squares over all q heads and over all k heads of each token
-    for (int t = 0; t < nt; ++t) {
-      float ss[2] = {0.f, 0.f};
-      for (int h = tid / LANES; h < p.hq + p.hk; h += kQkThreads / LANES) {
-        if (j >= chunks) continue;
-        const uint16_t* src = h < p.hq ? p.q + (t0 + t) * p.q_stride + h * p.d
-                                       : p.k + (t0 + t) * p.k_stride + (h - p.hq) * p.d;
-        float v[16];
-        unpack8<T>(ld16(src + 8 * c0), v);
-        unpack8<T>(ld16(src + 8 * c1), v + 8);
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) a = fmaf(v[i], v[i], a);
-        ss[h >= p.hq] += a;
-      }
-      ss[0] = warp_sum(ss[0]), ss[1] = warp_sum(ss[1]);
-      if (lane == 0) row_sum[0][t][warp] = ss[0], row_sum[1][t][warp] = ss[1];
-    }
-  }
-  __syncthreads();
-
-  const int total = nt * heads;  // (token, head) items, LANES threads each
-  const int rounds = (total + kQkThreads / LANES - 1) / (kQkThreads / LANES);
-  for (int r = 0; r < rounds; ++r) {  // uniform: the head sums below are warp-wide
-    const int item = r * (kQkThreads / LANES) + tid / LANES;
-    const bool live = item < total && j < chunks;
-    const int t = live ? item / heads : 0, h = live ? item - t * heads : 0;
-    const long long tok = t0 + t;
-    const int kind = h < p.hq ? 0 : h < p.hq + p.hk ? 1 : 2;  // q, k, v
-    const int g = kind == 0 ? h : kind == 1 ? h - p.hq : h - p.hq - p.hk;
-    const uint16_t* src = kind == 0   ? p.q + tok * p.q_stride
-                          : kind == 1 ? p.k + tok * p.k_stride
-                                      : p.v + tok * p.v_stride;
-    src += g * p.d;
-    uint16_t* dst = nullptr;
-    if (live) {
-      if (kind == 0) {
-        dst = p.q_out + tok * p.out_stride + g * p.d;
-      } else {
-        const unsigned slot = static_cast<unsigned>(p.slots[tok]);  // -1 is past the end too
-        if (slot < p.slots_end)
-          dst = (kind == 1 ? p.k_cache : p.v_cache) + static_cast<long long>(slot >> p.shift) * p.page_stride +
-                ((static_cast<long long>(g) << p.shift) + (slot & ((1u << p.shift) - 1))) * p.d;
-      }
-    }
+  // chunk c0 and its partner; the part past 2 * pairs starts at an even chunk
+  const int c0 = 8 * (!PAIRED && turned ? j : 2 * j);
+  const int c1 = 8 * (!PAIRED && turned ? j + (p.pairs >> 3) : 2 * j + 1);
+  // Parts of the heads: one per CTA, or all in turn where a norm over the row
+  // needs every head before any is written (q_out may be q).
+  for (int part = blockIdx.y; part * (threads / LANES) < p.hq + 2 * p.hk; part += gridDim.y) {
+    const int head = part * (threads / LANES) + tid / LANES;
+    const int kind = head < p.hq ? 0 : head < p.hq + p.hk ? 1 : 2;  // q, k, v
+    const int g = head - (kind == 0 ? 0 : kind == 1 ? p.hq : p.hq + p.hk);
+    const bool live = head < p.hq + 2 * p.hk && j < chunks;
+    const uint16_t* src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+    const long long step = kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride;
+    src += t0 * step + g * p.d;
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (live) a = ld16(src + 8 * c0), b = ld16(src + 8 * c1);
-    if (kind == 2) {
-      if (dst) st16(dst + 8 * c0, a), st16(dst + 8 * c1, b);
+    unsigned slot = 0;
+    if (live) {
+      a = ld16(src + c0), b = ld16(src + c1);
+      if (kind) slot = static_cast<unsigned>(p.slots[t0]);
     }
-    float x[16];
-    unpack8<T>(a, x);
-    unpack8<T>(b, x + 8);
+    uint4 wa, wb;  // this thread's weights
     if constexpr (NORM != VVLI_NORM_NONE) {
-      float ms;
-      if constexpr (NORM == VVLI_NORM_HEAD) {
-        ms = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ms = fmaf(x[i], x[i], ms);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, o);
-        ms /= static_cast<float>(p.d);
-      } else {
-        ms = 0.f;
-#pragma unroll
-        for (int w = 0; w < kQkThreads / 32; ++w) ms += row_sum[kind == 1][t][w];
-        ms /= static_cast<float>(kind == 1 ? p.hk : p.hq) * p.d;
-      }
-      const float scale = 1.0f / sqrtf(ms + p.eps);
-      const uint16_t* w = kind == 1 ? p.k_weight : p.q_weight;
-      if (NORM == VVLI_NORM_ROW && w) w += g * p.d;
-      float y[16];
-      if (w && live && kind != 2) {
-        unpack8<T>(ld16(w + 8 * c0), y);
-        unpack8<T>(ld16(w + 8 * c1), y + 8);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = x[i] * scale * y[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= scale;
+      const uint16_t* wp = kind == 1 ? p.k_weight : p.q_weight;
+      const uint32_t one = Pair16<T>::store(1.f, 1.f);
+      wa = wb = make_uint4(one, one, one, one);
+      if (wp && live && kind < 2) {
+        if (NORM == VVLI_NORM_ROW) wp += g * p.d;
+        wa = ld16(wp + c0), wb = ld16(wp + c1);
       }
     }
-    if (!dst || kind == 2) continue;  // the rest has no warp-wide step
-    if (turned) {
-      const float2* cs = turn + t * p.pairs + 8 * j;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 w = cs[i];
-        const float xa = p.interleaved ? x[2 * i] : x[i], xb = p.interleaved ? x[2 * i + 1] : x[i + 8];
-        const float ra = xa * w.x - xb * w.y, rb = xb * w.x + xa * w.y;
-        if (p.interleaved)
-          x[2 * i] = ra, x[2 * i + 1] = rb;
-        else
-          x[i] = ra, x[i + 8] = rb;
+    if (part == static_cast<int>(blockIdx.y)) {
+      for (int i = tid; i < nt * p.pairs; i += threads) {
+        const int t = i / p.pairs, f = i - t * p.pairs;
+        constexpr double kInvTwoPi = 0.15915494309189533576888;
+        const double turns = static_cast<double>(p.positions[t0 + t]) * p.inv_freq[f] * kInvTwoPi;
+        float s, c;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+        turn[i] = make_float2(c, s);
       }
+      if constexpr (NORM == VVLI_NORM_ROW) {
+        // square sums over all q heads and over all k heads of each token (whatever heads this CTA has)
+        for (int t = 0; t < nt; ++t) {
+          float ss[2] = {0.f, 0.f};
+          for (int h = tid / LANES; h < p.hq + p.hk; h += threads / LANES) {
+            if (j >= chunks) continue;
+            const uint16_t* row = h < p.hq ? p.q + (t0 + t) * p.q_stride + h * p.d
+                                           : p.k + (t0 + t) * p.k_stride + (h - p.hq) * p.d;
+            float v[16];
+            unpack8<T>(ld16(row + c0), v);
+            unpack8<T>(ld16(row + c1), v + 8);
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sq = fmaf(v[i], v[i], sq);
+            ss[h >= p.hq] += sq;
+          }
+          ss[0] = warp_sum(ss[0]), ss[1] = warp_sum(ss[1]);
+          if (lane == 0) row_sum[0][t][warp] = ss[0], row_sum[1][t][warp] = ss[1];
+        }
+      }
+      __syncthreads();
     }
-    st16(dst + 8 * c0, pack8<T>(x));
-    st16(dst + 8 * c1, pack8<T>(x + 8));
+
+    // the head's own threads: other heads of the warp may be values, which skip the sums
+    const unsigned head_mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
+    uint16_t* const out = p.q_out + t0 * p.out_stride + g * p.d;
+    uint16_t* const cache = kind == 1 ? p.k_cache : p.v_cache;
+    for (int t = 0; t < nt; ++t) {
+      uint4 na = make_uint4(0, 0, 0, 0), nb = na;
+      unsigned nslot = 0;
+      src += step;
+      if (live && t + 1 < nt) {  // the next token's, before this one's work
+        na = ld16(src + c0), nb = ld16(src + c1);
+        if (kind) nslot = static_cast<unsigned>(p.slots[t0 + t + 1]);
+      }
+      uint16_t* dst = nullptr;
+      if (live && kind == 0)
+        dst = out + t * p.out_stride;
+      else if (live && slot < p.slots_end)  // -1 is past the end too
+        dst = cache + static_cast<long long>(slot >> p.shift) * p.page_stride +
+              ((static_cast<long long>(g) << p.shift) + (slot & ((1u << p.shift) - 1))) * p.d;
+      if (kind < 2) {
+        float x[16];
+        unpack8<T>(a, x);
+        unpack8<T>(b, x + 8);
+        if constexpr (NORM != VVLI_NORM_NONE) {
+          float ms = 0.f;
+          if constexpr (NORM == VVLI_NORM_HEAD) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ms = fmaf(x[i], x[i], ms);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) ms += __shfl_xor_sync(head_mask, ms, o);
+          } else {
+            for (int u = 0; u < threads / 32; ++u) ms += row_sum[kind][t][u];
+          }
+          const float scale = rsqrtf(fmaf(ms, kind == 1 ? p.k_share : p.q_share, p.eps));
+          float w[16];
+          unpack8<T>(wa, w);
+          unpack8<T>(wb, w + 8);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= scale * w[i];
+        }
+        if (turned) {
+          const float4* cs = reinterpret_cast<const float4*>(turn + t * p.pairs + 8 * j);  // two pairs each
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 w2 = cs[i >> 1];
+            const float cw = i & 1 ? w2.z : w2.x, sw = i & 1 ? w2.w : w2.y;
+            float& xa = x[PAIRED ? 2 * i : i];
+            float& xb = x[PAIRED ? 2 * i + 1 : i + 8];
+            const float ra = xa * cw - xb * sw, rb = xb * cw + xa * sw;
+            xa = ra, xb = rb;
+          }
+        }
+        a = pack8<T>(x), b = pack8<T>(x + 8);
+      }
+      if (dst) st16(dst + c0, a), st16(dst + c1, b);
+      a = na, b = nb, slot = nslot;
+    }
   }
 }
 
@@ -236,27 +242,30 @@ std::string check_qk(const vvli_qk_rope_args* a) {
   return "";
 }
 
-template <class T, int NORM>
-cudaError_t queue_lanes(const QkDev& p, unsigned grid, size_t smem, cudaStream_t s) {
-  const int chunks = p.d >> 4;
-  if (chunks <= 1)
-    qk_rope_kernel<T, NORM, 1><<<grid, kQkThreads, smem, s>>>(p);
-  else if (chunks <= 2)
-    qk_rope_kernel<T, NORM, 2><<<grid, kQkThreads, smem, s>>>(p);
-  else if (chunks <= 4)
-    qk_rope_kernel<T, NORM, 4><<<grid, kQkThreads, smem, s>>>(p);
-  else if (chunks <= 8)
-    qk_rope_kernel<T, NORM, 8><<<grid, kQkThreads, smem, s>>>(p);
-  else
-    qk_rope_kernel<T, NORM, 16><<<grid, kQkThreads, smem, s>>>(p);
+template <class T, int NORM, bool PAIRED>
+cudaError_t queue_lanes(const QkDev& p, size_t smem, cudaStream_t s) {
+  int lanes = 1;
+  while (lanes < p.d >> 4) lanes *= 2;
+  // all heads in one CTA if it can hold them, else in CTAs of equal shares
+  const int heads = p.hq + 2 * p.hk, most = kQkMaxThreads / lanes;
+  const int parts = (heads + most - 1) / most, each = (heads + parts - 1) / parts;
+  const int threads = (each * lanes + 31) & ~31;
+  const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, NORM == VVLI_NORM_ROW ? 1 : (heads + threads / lanes - 1) / (threads / lanes));
+  switch (lanes) {
+    case 1: qk_rope_kernel<T, NORM, 1, PAIRED><<<grid, threads, smem, s>>>(p); break;
+    case 2: qk_rope_kernel<T, NORM, 2, PAIRED><<<grid, threads, smem, s>>>(p); break;
+    case 4: qk_rope_kernel<T, NORM, 4, PAIRED><<<grid, threads, smem, s>>>(p); break;
+    case 8: qk_rope_kernel<T, NORM, 8, PAIRED><<<grid, threads, smem, s>>>(p); break;
+    default: qk_rope_kernel<T, NORM, 16, PAIRED><<<grid, threads, smem, s>>>(p); break;
+  }
   return cudaGetLastError();
 }
 
-template <class T>
-cudaError_t queue_norm(const QkDev& p, int norm, unsigned grid, size_t smem, cudaStream_t s) {
-  return norm == VVLI_NORM_NONE   ? queue_lanes<T, VVLI_NORM_NONE>(p, grid, smem, s)
-         : norm == VVLI_NORM_HEAD ? queue_lanes<T, VVLI_NORM_HEAD>(p, grid, smem, s)
-                                  : queue_lanes<T, VVLI_NORM_ROW>(p, grid, smem, s);
+template <class T, bool PAIRED>
+cudaError_t queue_norm(const QkDev& p, int norm, size_t smem, cudaStream_t s) {
+  return norm == VVLI_NORM_NONE   ? queue_lanes<T, VVLI_NORM_NONE, PAIRED>(p, smem, s)
+         : norm == VVLI_NORM_HEAD ? queue_lanes<T, VVLI_NORM_HEAD, PAIRED>(p, smem, s)
+                                  : queue_lanes<T, VVLI_NORM_ROW, PAIRED>(p, smem, s);
 }
 
 cudaError_t queue_qk(const vvli_qk_rope_args& a, cudaStream_t s) {
@@ -266,22 +275,26 @@ cudaError_t queue_qk(const vvli_qk_rope_args& a, cudaStream_t s) {
   p.d = static_cast<int>(a.head_dim), p.pairs = static_cast<int>(a.rotary_pairs);
   p.shift = 4;
   while ((1u << p.shift) < a.page_size) ++p.shift;
-  p.interleaved = a.interleaved != 0;
   p.slots_end = static_cast<unsigned>(a.pages) << p.shift;
   p.page_stride = static_cast<long long>(a.page_stride), p.q_stride = static_cast<long long>(a.q_stride);
   p.k_stride = static_cast<long long>(a.k_stride), p.v_stride = static_cast<long long>(a.v_stride);
   p.out_stride = static_cast<long long>(a.out_stride);
   p.eps = a.eps;
+  const bool row = a.norm == VVLI_NORM_ROW;
+  p.q_share = 1.0f / static_cast<float>(row ? p.hq * p.d : p.d);
+  p.k_share = 1.0f / static_cast<float>(row ? p.hk * p.d : p.d);
   p.q = static_cast<const uint16_t*>(a.q), p.k = static_cast<const uint16_t*>(a.k);
   p.v = static_cast<const uint16_t*>(a.v), p.q_out = static_cast<uint16_t*>(a.q_out);
   p.k_cache = static_cast<uint16_t*>(a.k_cache), p.v_cache = static_cast<uint16_t*>(a.v_cache);
   p.q_weight = static_cast<const uint16_t*>(a.q_weight), p.k_weight = static_cast<const uint16_t*>(a.k_weight);
   p.positions = a.positions, p.slots = a.slots, p.inv_freq = a.inv_freq;
-  p.per_cta = 1;
-  const unsigned grid = static_cast<unsigned>((p.tokens + p.per_cta - 1) / p.per_cta);
+  // Few tokens are spread over the SMs; many share a CTA's table and prologue.
+  p.per_cta = p.tokens <= 256 ? 1 : p.tokens <= 1024 ? 2 : kQkMaxTokens;
   const size_t smem = static_cast<size_t>(p.per_cta) * p.pairs * sizeof(float2);
-  return a.dtype == VVLI_BF16 ? queue_norm<__nv_bfloat16>(p, a.norm, grid, smem, s)
-                              : queue_norm<__half>(p, a.norm, grid, smem, s);
+  if (a.dtype == VVLI_BF16)
+    return a.interleaved ? queue_norm<__nv_bfloat16, true>(p, a.norm, smem, s)
+                         : queue_norm<__nv_bfloat16, false>(p, a.norm, smem, s);
+  return a.interleaved ? queue_norm<__half, true>(p, a.norm, smem, s) : queue_norm<__half, false>(p, a.norm, smem, s);
 }
 
 }  // namespace

@@ -12,8 +12,8 @@
 // weights of the one row that is drawn from, a contiguous slice per CTA and
 // per warp, in 64 bits: a cumulative sum of 10^5 fp32 terms rounded to 32 bits
 // would move the drawn index.  The CTAs exchange their slice sums through
-// distributed shared memory, the warp whose slice holds the threshold walks it
-// once more (from L2) with a warp scan.  Bound: HBM, one row of the target and,
+// distributed shared memory, and the CTA with the threshold goes over the one
+// warp slice that holds it once more (from L2), a short run per thread.  Bound: HBM, one row of the target and,
 // when a draft was rejected, one of the draft model per request.
 #include <algorithm>
 #include <climits>
@@ -28,7 +28,7 @@ namespace {
 constexpr int kVerThreads = 256;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerCluster = 8;
-constexpr int kVerUnroll = 8;  // loads in flight per lane and row
+constexpr int kVerUnroll = 4;  // loads in flight per lane and row
 
 VVLI_DEV uint32_t ver_cluster_rank() {
   uint32_t r;
@@ -51,10 +51,19 @@ struct Weights {
   const float* t;
   const float* d;
   int skip;
-  VVLI_DEV double at(int i) const {
-    double w = static_cast<double>(t[i]);
-    if (d) w -= static_cast<double>(d[i]);
+  VVLI_DEV double of(float a, float b, int i) const {
+    const double w = static_cast<double>(a) - static_cast<double>(b);
     return w > 0.0 && i != skip ? w : 0.0;  // NaN: 0
+  }
+  VVLI_DEV double at(int i) const { return of(t[i], d ? d[i] : 0.f, i); }
+  // Four values from i on, zeros from `end` on (i a multiple of 4, rows 16-byte aligned).
+  VVLI_DEV float4 load4(const float* row, int i, int end) const {
+    if (!row || i >= end) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i + 4 <= end) return *reinterpret_cast<const float4*>(row + i);
+    return make_float4(row[i], i + 1 < end ? row[i + 1] : 0.f, i + 2 < end ? row[i + 2] : 0.f, 0.f);
+  }
+  VVLI_DEV double of4(const float4& a, const float4& b, int i) const {
+    return (of(a.x, b.x, i) + of(a.y, b.y, i + 1)) + (of(a.z, b.z, i + 2) + of(a.w, b.w, i + 3));
   }
 };
 
@@ -64,8 +73,11 @@ VVLI_DEV double warp_sum_f64(double v) {
   return v;
 }
 
+// VEC: 4 when every row starts on a 16-byte boundary, else 1.
+template <int VEC>
 __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_args p) {
   __shared__ double warp_part[kVerWarps];
+  __shared__ double scan_part[kVerWarps];
   __shared__ double cta_part[2];  // this CTA's slice sum, by attempt (read by the cluster)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / kVerCluster;
@@ -111,7 +123,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
       w.skip = p.tokens[row + 1];
   }
   // contiguous slices: CTA `rank` of the cluster, warp `warp` of the CTA
-  const int per_warp = (V + kVerCluster * kVerWarps - 1) / (kVerCluster * kVerWarps);
+  const int per_warp = ((V + kVerCluster * kVerWarps - 1) / (kVerCluster * kVerWarps) + 3) & ~3;  // V <= 2^30
   const long long first = static_cast<long long>(rank * kVerWarps + warp) * per_warp;
   const int s0 = static_cast<int>(min(first, static_cast<long long>(V)));
   const int s1 = static_cast<int>(min(first + per_warp, static_cast<long long>(V)));
@@ -120,12 +132,25 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
   double thr = 0.0;
   for (int attempt = 0; attempt < 2; ++attempt) {
     double sum = 0.0;
-    for (int i0 = s0 + lane; i0 < s1; i0 += 32 * kVerUnroll) {
-      double x[kVerUnroll];
+    if constexpr (VEC == 4) {
+      for (int i0 = s0 + 4 * lane; i0 < s1; i0 += 128 * kVerUnroll) {
+        float4 x[kVerUnroll], y[kVerUnroll];
 #pragma unroll
-      for (int u = 0; u < kVerUnroll; ++u) x[u] = i0 + 32 * u < s1 ? w.at(i0 + 32 * u) : 0.0;
+        for (int u = 0; u < kVerUnroll; ++u) x[u] = w.load4(w.t, i0 + 128 * u, s1), y[u] = w.load4(w.d, i0 + 128 * u, s1);
 #pragma unroll
-      for (int u = 0; u < kVerUnroll; ++u) sum += x[u];
+        for (int u = 0; u < kVerUnroll; ++u) sum += w.of4(x[u], y[u], i0 + 128 * u);
+      }
+    } else {
+      for (int i0 = s0 + lane; i0 < s1; i0 += 32 * kVerUnroll) {
+        float x[kVerUnroll], y[kVerUnroll];
+#pragma unroll
+        for (int u = 0; u < kVerUnroll; ++u) {
+          const int i = i0 + 32 * u;
+          x[u] = i < s1 ? w.t[i] : 0.f, y[u] = w.d && i < s1 ? w.d[i] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kVerUnroll; ++u) sum += w.of(x[u], y[u], i0 + 32 * u);
+      }
     }
     mine = warp_sum_f64(sum);
     if (lane == 0) warp_part[warp] = mine;
@@ -168,28 +193,60 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
     run += part;
   }
   if (cw < 0) cw = last, wb = last_before;
-  if (warp != cw) return;
-  // the smallest index of this slice whose cumulative weight exceeds thr, or its last with any weight
-  int best = 0, some = -1;
-  bool found = false;
-  run = wb;
-  for (int i0 = s0; i0 < s1 && !found; i0 += 32) {
-    const int i = i0 + lane;
-    const double x = i < s1 ? w.at(i) : 0.0;
-    double c = x;
+  // That slice again, by the whole CTA: a contiguous run per thread, its sum, a
+  // scan over the CTA, and the thread whose run holds the threshold walks it.
+  const long long c_first = static_cast<long long>(rank * kVerWarps + cw) * per_warp;
+  const int c0 = static_cast<int>(min(c_first, static_cast<long long>(V)));
+  const int c1 = static_cast<int>(min(c_first + per_warp, static_cast<long long>(V)));
+  const int per = (c1 - c0 + kVerThreads - 1) / kVerThreads;
+  const int b0 = min(c0 + tid * per, c1), b1 = min(b0 + per, c1);
+  double sum = 0.0;
+  for (int i0 = b0; i0 < b1; i0 += kVerUnroll) {
+    float x[kVerUnroll], y[kVerUnroll];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, c, o);
-      if (lane >= o) c += y;
+    for (int u = 0; u < kVerUnroll; ++u) {
+      const int i = i0 + u;
+      x[u] = i < b1 ? w.t[i] : 0.f, y[u] = w.d && i < b1 ? w.d[i] : 0.f;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && run + c > thr);
-    const unsigned any = __ballot_sync(0xffffffffu, x > 0.0);
-    if (hit) best = i0 + __ffs(hit) - 1, found = true;
-    if (any) some = i0 + 31 - __clz(any);
-    run += __shfl_sync(0xffffffffu, c, 31);
+#pragma unroll
+    for (int u = 0; u < kVerUnroll; ++u) sum += w.of(x[u], y[u], i0 + u);
   }
-  if (!found && some >= 0) best = some;
-  if (lane == 0) p.out_tokens[row] = best;
+  double c = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, c, o);
+    if (lane >= o) c += y;
+  }
+  if (lane == 31) scan_part[warp] = c;
+  __syncthreads();
+  double lead = wb;
+#pragma unroll
+  for (int u = 0; u < kVerWarps; ++u)
+    if (u < warp) lead += scan_part[u];
+  // the first thread whose run passes the threshold, else the last with any weight
+  __shared__ int hit_s[kVerWarps], any_s[kVerWarps];
+  const unsigned hit = __ballot_sync(0xffffffffu, sum > 0.0 && lead + c > thr);
+  const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+  if (lane == 0) {
+    hit_s[warp] = hit ? warp * 32 + __ffs(hit) - 1 : INT_MAX;
+    any_s[warp] = any ? warp * 32 + 31 - __clz(any) : -1;
+  }
+  __syncthreads();
+  int owner = INT_MAX, some = -1;
+#pragma unroll
+  for (int u = 0; u < kVerWarps; ++u) owner = min(owner, hit_s[u]), some = max(some, any_s[u]);
+  if (owner == INT_MAX) owner = max(some, 0);
+  if (tid != owner) return;
+  int best = c0;  // no weight at all: the slice's first index (0: the draw falls to the first slice)
+  run = lead + c - sum;
+  for (int i = b0; i < b1; ++i) {
+    const double x = w.at(i);
+    if (x <= 0.0) continue;
+    best = i;
+    run += x;
+    if (run > thr) break;
+  }
+  p.out_tokens[row] = best;
 }
 
 std::string check_verify(const vvli_verify_args* a) {
@@ -220,7 +277,9 @@ cudaError_t queue_verify(const vvli_verify_args& a, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_kernel, a);
+  const bool vec = aligned_to(a.target, 16) && a.target_stride % 4 == 0 &&
+                   (!a.draft || (aligned_to(a.draft, 16) && a.draft_stride % 4 == 0));
+  return vec ? cudaLaunchKernelEx(&cfg, verify_kernel<4>, a) : cudaLaunchKernelEx(&cfg, verify_kernel<1>, a);
 }
 
 }  // namespace

@@ -32,8 +32,15 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _NORMS = {"none": 0, None: 0, "head": 1, "row": 2}
 
 
-def _stream(device: torch.device, stream) -> int:
-    return (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+# The wrappers' own time counts beside kernels of a few microseconds: devices are
+# compared by index, and the current stream's handle comes straight from torch's
+# C module (torch.cuda.current_stream builds an object for it, 2 us).
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _stream(index: int, stream) -> int:
+    return _current_stream(index) if stream is None else stream.cuda_stream
 
 
 def _empty(shape, dtype, device, stream):
@@ -44,36 +51,43 @@ def _empty(shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _ints(who: str, name: str, t, device, n=None):
-    """t as a contiguous int32 tensor of `device` with at least n entries."""
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or (n is not None and t.numel() < n):
-        raise ValueError(f"{who}: {name} must be a contiguous int32 tensor on {device}"
-                         + (f" with at least {n} entries" if n is not None else ""))
+def _empty_like(x, stream):
+    if stream is None and x.is_contiguous():
+        return torch.empty_like(x)
+    return _empty(x.shape, x.dtype, x.device, stream)
+
+
+def _ints(who: str, name: str, t, index: int, n: int = 0) -> int:
+    """Address of a contiguous int32 tensor of CUDA device `index` with at least n entries."""
+    if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{who}: {name} must be a contiguous int32 tensor on cuda:{index} with at least {n} entries")
     return t.data_ptr()
 
 
-def _cache_layout(who: str, k_cache, v_cache, heads: int, d: int, dtype, device):
+def _cache_layout(who: str, k_cache, v_cache, heads: int, d: int, dtype, index: int):
     """(pages, page_size, page_stride) of a pair of caches."""
     shape, strides = k_cache.shape, k_cache.stride()
-    if k_cache.dim() != 4 or v_cache.shape != shape or v_cache.stride() != strides:
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
         raise ValueError(f"{who}: k_cache and v_cache must be alike, [pages][kv heads][page_size][head_dim]")
-    if shape[1] != heads or shape[3] != d or strides[1:] != (shape[2] * d, d, 1):
+    pages, h, page_size, dc = shape
+    apart, s1, s2, s3 = strides
+    if h != heads or dc != d or s3 != 1 or s2 != d or (s1 != page_size * d and h > 1):
         raise ValueError(f"{who}: the caches' pages must be contiguous [{heads}][page_size][{d}]")
-    for c in (k_cache, v_cache):
-        if c.dtype != dtype or c.device != device:
-            raise ValueError(f"{who}: the caches must be {dtype} on {device}")
-    return shape[0], shape[2], strides[0] if shape[0] > 1 else shape[1] * shape[2] * d
+    if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or k_cache.get_device() != index
+            or v_cache.get_device() != index):
+        raise ValueError(f"{who}: the caches must be {dtype} on cuda:{index}")
+    return pages, page_size, apart if pages > 1 else h * page_size * d
 
 
-def _heads(who: str, name: str, x, dtype, device):
-    """Row stride of a [tokens][heads][d] tensor whose rows are contiguous."""
-    if x.dim() != 3 or x.dtype != dtype or x.device != device:
-        raise ValueError(f"{who}: {name} must be a [tokens][heads][head_dim] {dtype} tensor on {device}")
-    n, h, d = x.shape
-    s = x.stride()
-    if (d > 1 and s[2] != 1) or (h > 1 and s[1] != d):
+def _heads(who: str, name: str, x, shape, dtype, index: int) -> int:
+    """Row stride of a tensor of the given [tokens][heads][d] shape whose rows are contiguous."""
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+        raise ValueError(f"{who}: {name} must be a {list(shape)} {dtype} tensor on cuda:{index}")
+    apart, sh, sd = x.stride()
+    n, h, d = shape
+    if (sd != 1 and d > 1) or (sh != d and h > 1):
         raise ValueError(f"{who}: the rows of {name} must be contiguous")
-    return s[0] if n > 1 else h * d
+    return apart if n > 1 else h * d
 
 
 class StepPlan(NamedTuple):
@@ -97,32 +111,31 @@ def plan_step(context, new, owned, block_table, free_pages, free_count, page_siz
     entries are free.  max_tokens: rows of the step (a captured step may have
     more than are used).  With inplace=True, owned and free_count are updated
     themselves (and are the plan's)."""
-    who, dev = "plan_step", context.device
-    if dev.type != "cuda":
+    who, dev = "plan_step", context.get_device()
+    if dev < 0:
         raise ValueError("plan_step: context must be a CUDA tensor")
     B = context.numel()
     if block_table.dim() != 2 or block_table.shape[0] < B:
         raise ValueError("plan_step: block_table must be [requests][width]")
-    max_tokens = int(max_tokens)
     if max_tokens < 0:
         raise ValueError("plan_step: max_tokens must be >= 0")
-    sizes = [B + 1, B, max_tokens, max_tokens, B, 1, B]
-    buf = _empty((sum(sizes),), torch.int32, dev, stream)
-    at = buf.data_ptr()
-    ptr = []
-    for n in sizes:
-        ptr.append(at)
-        at += 4 * n
+    sizes = (B + 1, B, max_tokens, max_tokens, B, 1, B)
+    buf = _empty(4 * B + 2 * max_tokens + 2, torch.int32, context.device, stream)
+    cu = buf.data_ptr()
+    seq = cu + 4 * (B + 1)
+    pos = seq + 4 * B
+    slots = pos + 4 * max_tokens
+    own = slots + 4 * max_tokens
     own_in, free_in = _ints(who, "owned", owned, dev, B), _ints(who, "free_count", free_count, dev, 1)
     a = _abi.CPagedPlanArgs(
-        B, int(page_size), free_pages.numel(), block_table.shape[1], max_tokens, _ints(who, "context", context, dev),
+        B, page_size, free_pages.numel(), block_table.shape[1], max_tokens, _ints(who, "context", context, dev),
         _ints(who, "new", new, dev, B), own_in, _ints(who, "block_table", block_table, dev),
-        _ints(who, "free_pages", free_pages, dev), free_in, ptr[0], ptr[1], ptr[2], ptr[3],
-        own_in if inplace else ptr[4], free_in if inplace else ptr[5], ptr[6])
-    check(_abi.lib().vvli_cuda_paged_plan(dev.index, ctypes.byref(a), _stream(dev, stream)))
-    out = buf.split(sizes)
+        _ints(who, "free_pages", free_pages, dev), free_in, cu, seq, pos, slots, own_in if inplace else own,
+        free_in if inplace else own + 4 * B, own + 4 * B + 4)
+    check(_abi.lib().vvli_cuda_paged_plan(dev, ctypes.byref(a), _stream(dev, stream)))
+    out = buf.split_with_sizes(sizes)
     if inplace:
-        out = out[:4] + (owned, free_count, out[6])
+        out = (*out[:4], owned, free_count, out[6])
     return StepPlan(*out)
 
 
@@ -137,42 +150,47 @@ def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_fre
     rotary pair, None for no rotation.  slots and positions: int32 [tokens]; a
     slot of -1 writes no k and v.  Returns the normed, turned q: ``out``
     (which may be q) or a new tensor."""
-    who, dev, dtype = "qk_norm_rope_write", q.device, q.dtype
-    if dev.type != "cuda" or dtype not in _DTYPES:
-        raise ValueError("qk_norm_rope_write: q must be a bf16 or fp16 CUDA tensor")
+    who, dev, dtype = "qk_norm_rope_write", q.get_device(), q.dtype
+    if dev < 0 or dtype not in _DTYPES or q.dim() != 3 or k.dim() != 3:
+        raise ValueError("qk_norm_rope_write: q and k must be [tokens][heads][head_dim] bf16 or fp16 CUDA tensors")
     if norm not in _NORMS:
         raise ValueError("qk_norm_rope_write: norm must be 'head', 'row' or 'none'")
-    qs, ks, vs = (_heads(who, n, x, dtype, dev) for n, x in (("q", q), ("k", k), ("v", v)))
-    T, hq, d = q.shape
+    T, hq, d = shape = q.shape
     hk = k.shape[1]
-    if k.shape != (T, hk, d) or v.shape != (T, hk, d):
-        raise ValueError("qk_norm_rope_write: k and v must be [tokens][kv heads][head_dim] with q's tokens and head_dim")
+    qs = _heads(who, "q", q, shape, dtype, dev)
+    ks = _heads(who, "k", k, (T, hk, d), dtype, dev)
+    vs = _heads(who, "v", v, (T, hk, d), dtype, dev)
     pages, page_size, page_stride = _cache_layout(who, k_cache, v_cache, hk, d, dtype, dev)
-    pairs = 0
+    pairs = freq = pos = qw = kw = None
     if inv_freq is not None:
-        pairs = inv_freq.numel()
-        if inv_freq.dtype != torch.float64 or inv_freq.device != dev or not inv_freq.is_contiguous():
-            raise ValueError(f"qk_norm_rope_write: inv_freq must be a contiguous float64 tensor on {dev}")
+        if inv_freq.dtype is not torch.float64 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+            raise ValueError(f"qk_norm_rope_write: inv_freq must be a contiguous float64 tensor on cuda:{dev}")
         if positions is None:
             raise ValueError("qk_norm_rope_write: a rotation needs positions")
-    for name, w, n in (("q_weight", q_weight, hq), ("k_weight", k_weight, hk)):
-        n = n * d if norm == "row" else d
-        if w is not None and (w.dtype != dtype or w.device != dev or w.numel() != n or not w.is_contiguous()):
-            raise ValueError(f"qk_norm_rope_write: {name} must be {n} contiguous {dtype} values on {dev}")
+        pairs, freq = inv_freq.numel(), inv_freq.data_ptr()
+    if positions is not None:
+        pos = _ints(who, "positions", positions, dev, T)
+    if q_weight is not None:
+        qw = _norm_weight("q_weight", q_weight, hq * d if norm == "row" else d, dtype, dev)
+    if k_weight is not None:
+        kw = _norm_weight("k_weight", k_weight, hk * d if norm == "row" else d, dtype, dev)
     if out is None:
-        out = _empty((T, hq, d), dtype, dev, stream)
-    elif out.shape != q.shape:
-        raise ValueError("qk_norm_rope_write: out must have q's shape")
+        out, os = _empty(shape, dtype, q.device, stream), hq * d
+    else:
+        os = _heads(who, "out", out, shape, dtype, dev)
     a = _abi.CQkRopeArgs(
-        T, hq, hk, d, pairs, page_size, pages, page_stride, qs, ks, vs, _heads(who, "out", out, dtype, dev),
-        _DTYPES[dtype], _NORMS[norm], int(bool(interleaved)), float(eps), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(),
-        None if positions is None else _ints(who, "positions", positions, dev, T), _ints(who, "slots", slots, dev, T),
-        None if inv_freq is None else inv_freq.data_ptr())
+        T, hq, hk, d, pairs or 0, page_size, pages, page_stride, qs, ks, vs, os, _DTYPES[dtype], _NORMS[norm],
+        1 if interleaved else 0, eps, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), qw, kw, pos, _ints(who, "slots", slots, dev, T), freq)
     if T:
-        check(_abi.lib().vvli_cuda_qk_rope_write(dev.index, ctypes.byref(a), _stream(dev, stream)))
+        check(_abi.lib().vvli_cuda_qk_rope_write(dev, ctypes.byref(a), _stream(dev, stream)))
     return out
+
+
+def _norm_weight(name: str, w, n: int, dtype, index: int) -> int:
+    if w.dtype is not dtype or w.get_device() != index or w.numel() != n or not w.is_contiguous():
+        raise ValueError(f"qk_norm_rope_write: {name} must be {n} contiguous {dtype} values on cuda:{index}")
+    return w.data_ptr()
 
 
 class PagedAttention:
@@ -197,6 +215,10 @@ class PagedAttention:
         if device is None:
             device = torch.cuda.current_device()
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("PagedAttention: device must be a CUDA device")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         if alibi is not None and (alibi.dtype != torch.float32 or alibi.numel() != q_heads or not alibi.is_contiguous()
                                   or alibi.device != self.device):
             raise ValueError(f"PagedAttention: alibi must be {q_heads} contiguous float32 values on {self.device}")
@@ -206,19 +228,19 @@ class PagedAttention:
         self.softcap, self.window = float(softcap), int(window)
         if self.window < 0:
             raise ValueError("PagedAttention: window must be >= 0")
+        self._type, self._alibi = _DTYPES[dtype], None if alibi is None else alibi.data_ptr()
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._ws[:4].zero_()
+        self._ws_at, self._ws_bytes = self._ws.data_ptr(), need
 
     def __call__(self, q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: int, out=None, lse=False, stream=None):
         """q: [rows][q_heads][head_dim]; block_table: int32 [requests][width]; cu_new: int32 [requests + 1] and seq_len:
         int32 [requests], as plan_step gives them; max_new: the longest request's new tokens (picks the kernel).
         Returns out ([rows][q_heads][head_dim], new unless given; rows of no request are not written), and with
         lse=True, or a float32 [rows][q_heads] tensor for it, (out, lse)."""
-        who, dev, dtype = "PagedAttention", self.device, self.dtype
-        qs = _heads(who, "q", q, dtype, dev)
-        T, hq, d = q.shape
-        if hq != self.q_heads or d != self.head_dim:
-            raise ValueError(f"PagedAttention: q must be [rows][{self.q_heads}][{self.head_dim}]")
+        who, dev, dtype = "PagedAttention", self.device.index, self.dtype
+        T, hq, d = shape = (q.shape[0], self.q_heads, self.head_dim)
+        qs = _heads(who, "q", q, shape, dtype, dev)
         pages, page_size, page_stride = _cache_layout(who, k_cache, v_cache, self.kv_heads, d, dtype, dev)
         if page_size != self.page_size:
             raise ValueError(f"PagedAttention: the caches' pages must have {self.page_size} positions")
@@ -226,22 +248,23 @@ class PagedAttention:
         if block_table.dim() != 2 or block_table.shape[0] < B:
             raise ValueError("PagedAttention: block_table must be [requests][width]")
         if out is None:
-            out = _empty((T, hq, d), dtype, dev, stream)
-        elif out.shape != q.shape:
-            raise ValueError("PagedAttention: out must have q's shape")
+            out, os = _empty_like(q, stream), hq * d
+        else:
+            os = _heads(who, "out", out, shape, dtype, dev)
+        lp = None
         if lse is True:
-            lse = _empty((T, hq), torch.float32, dev, stream)
-        elif lse is not False and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (T, hq)
-                                   or not lse.is_contiguous()):
-            raise ValueError(f"PagedAttention: lse must be a contiguous [{T}][{hq}] float32 tensor on {dev}")
+            lse = _empty((T, hq), torch.float32, self.device, stream)
+            lp = lse.data_ptr()
+        elif lse is not False:
+            if lse.dtype is not torch.float32 or lse.get_device() != dev or lse.shape != (T, hq) or not lse.is_contiguous():
+                raise ValueError(f"PagedAttention: lse must be a contiguous [{T}][{hq}] float32 tensor on cuda:{dev}")
+            lp = lse.data_ptr()
         a = _abi.CPagedAttnArgs(
-            B, T, hq, self.kv_heads, d, page_size, pages, page_stride, block_table.shape[1], qs,
-            _heads(who, "out", out, dtype, dev), max(0, int(max_new)), self.window, _DTYPES[dtype], self.scale, self.softcap, 0,
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-            None if lse is False else lse.data_ptr(), None if self.alibi is None else self.alibi.data_ptr(),
-            _ints(who, "block_table", block_table, dev), _ints(who, "cu_new", cu_new, dev, B + 1),
-            _ints(who, "seq_len", seq_len, dev), self._ws.data_ptr(), self._ws.numel())
-        check(_abi.lib().vvli_cuda_paged_attention(dev.index, ctypes.byref(a), _stream(dev, stream)))
+            B, T, hq, self.kv_heads, d, page_size, pages, page_stride, block_table.shape[1], qs, os, max(0, max_new),
+            self.window, self._type, self.scale, self.softcap, 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), lp, self._alibi, _ints(who, "block_table", block_table, dev),
+            _ints(who, "cu_new", cu_new, dev, B + 1), _ints(who, "seq_len", seq_len, dev), self._ws_at, self._ws_bytes)
+        check(_abi.lib().vvli_cuda_paged_attention(dev, ctypes.byref(a), _stream(dev, stream)))
         return out if lse is False else (out, lse)
 
     def status(self) -> int:

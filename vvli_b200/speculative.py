@@ -17,11 +17,17 @@ from .errors import check
 from .paged import _empty, _ints, _stream
 
 
-def _rows_of(name: str, x, dev, shape=None):
-    if x.dtype != torch.float32 or x.device != dev or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (
-            shape is not None and x.shape != shape):
-        raise ValueError(f"verify_drafts: {name} must be a [rows][vocab] float32 tensor on {dev} with contiguous rows")
+def _rows_of(name: str, x, index: int, shape=None) -> int:
+    if x.dtype is not torch.float32 or x.get_device() != index or x.dim() != 2 or (
+            x.stride(1) != 1 and x.shape[1] > 1) or (shape is not None and x.shape != shape):
+        raise ValueError(f"verify_drafts: {name} must be a [rows][vocab] float32 tensor on cuda:{index} with contiguous rows")
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _uniform(name: str, u, n: int, index: int) -> int:
+    if u.dtype is not torch.float32 or u.get_device() != index or u.numel() < n or not u.is_contiguous():
+        raise ValueError(f"verify_drafts: {name} must be {n} contiguous float32 values on cuda:{index}")
+    return u.data_ptr()
 
 
 def verify_drafts(target, draft, tokens, cu_rows, u_accept, u_sample, stream=None):
@@ -35,25 +41,22 @@ def verify_drafts(target, draft, tokens, cu_rows, u_accept, u_sample, stream=Non
     Returns (accepted [requests], out [rows]) int32: out holds the accepted
     drafts from cu_rows[b] on, then the drawn token, then -1; rows of no
     request are not written."""
-    dev = target.device
-    if dev.type != "cuda":
+    dev = target.get_device()
+    if dev < 0:
         raise ValueError("verify_drafts: target must be a CUDA tensor")
     ts = _rows_of("target", target, dev)
     ds = 0 if draft is None else _rows_of("draft", draft, dev, target.shape)
     T, V = target.shape
     B = u_sample.numel()
-    for name, u, n in (("u_accept", u_accept, T), ("u_sample", u_sample, B)):
-        if u.dtype != torch.float32 or u.device != dev or u.numel() < n or not u.is_contiguous():
-            raise ValueError(f"verify_drafts: {name} must be {n} contiguous float32 values on {dev}")
-    buf = _empty((B + T,), torch.int32, dev, stream)
+    ua, us = _uniform("u_accept", u_accept, T, dev), _uniform("u_sample", u_sample, B, dev)
+    tok, cu = _ints("verify_drafts", "tokens", tokens, dev, T), _ints("verify_drafts", "cu_rows", cu_rows, dev, B + 1)
+    buf = _empty(B + T, torch.int32, target.device, stream)
     if T == 0:  # no request has a row
         with torch.cuda.stream(stream):  # None: the current one
             buf.zero_()
-        return buf[:B], buf[B:]
-    at = buf.data_ptr()
-    a = _abi.CVerifyArgs(B, T, V, ts, ds, target.data_ptr(), None if draft is None else draft.data_ptr(),
-                         _ints("verify_drafts", "tokens", tokens, dev, T),
-                         _ints("verify_drafts", "cu_rows", cu_rows, dev, B + 1), u_accept.data_ptr(),
-                         u_sample.data_ptr(), at, at + 4 * B)
-    check(_abi.lib().vvli_cuda_verify_drafts(dev.index, ctypes.byref(a), _stream(dev, stream)))
-    return buf[:B], buf[B:]
+    else:
+        at = buf.data_ptr()
+        a = _abi.CVerifyArgs(B, T, V, ts, ds, target.data_ptr(), None if draft is None else draft.data_ptr(), tok, cu, ua, us,
+                             at, at + 4 * B)
+        check(_abi.lib().vvli_cuda_verify_drafts(dev, ctypes.byref(a), _stream(dev, stream)))
+    return buf.split_with_sizes((B, T))
