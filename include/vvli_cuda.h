@@ -582,9 +582,9 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * q head g uses kv head g / (q_heads / kv_heads).  A row that sees no key
  * (p < 0) gets out 0 and lse -inf; rows from cu_new[requests] on are left as
  * they were.  What the cache holds past a request's seq_len is never used,
- * whatever its bits.  Keys whose table entry is outside [0, pages), or past
- * table_width, count as zero keys and values.  cu_new must not decrease and
- * is cut at `tokens`.  Products of 16-bit values summed in fp32; the
+ * whatever its bits.  Keys whose table entry is outside [0, pages) count as
+ * zero keys and values.  cu_new must not decrease and is cut at `tokens`,
+ * seq_len at table_width * page_size.  Products of 16-bit values summed in fp32; the
  * probabilities enter the second product rounded to the 16-bit type, relative
  * to the row's largest score; results do not depend on timing.
  * `max_new` is the longest request's new tokens as far as the caller knows:

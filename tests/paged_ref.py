@@ -59,12 +59,13 @@ def attention(q, k_cache, v_cache, table, cu_new, seq_len, scale, window=0, soft
     out = torch.full((T, hq, d), math.nan, dtype=torch.float64)
     lse = torch.full((T, hq), math.nan, dtype=torch.float64)
     for b, end in enumerate(seq_len):
+        end = min(end, len(table[b]) * page)
         r0, r1 = min(cu_new[b], T), min(max(cu_new[b], cu_new[b + 1]), T)
         n = cu_new[b + 1] - cu_new[b]
         k = torch.zeros(hk, max(end, 0), d, dtype=torch.float64)
         v = torch.zeros_like(k)
         for j in range(-(-max(end, 0) // page)):
-            at = int(table[b][j]) if j < len(table[b]) else -1
+            at = int(table[b][j])
             if 0 <= at < pages:
                 m = min(page, end - j * page)
                 k[:, j * page:j * page + m] = k_cache[at, :, :m].double()

@@ -133,12 +133,12 @@ def test_max_new_only_picks_the_kernel(torch, max_new):
 
 @pytest.mark.parametrize("max_new", [1, 10**6])
 def test_empty_rows_bad_pages_and_rows_behind(torch, max_new):
-    # seq_len 0 (an unserved request), fewer keys than rows, entries outside the cache, a short table
+    # seq_len 0 (an unserved request), fewer keys than rows, entries outside the cache, lengths past the table
     lens = [(0, 3), (2, 5), (-4, 2), (100, 4), (200, 1), (150, 2)]
     inp = list(make(torch, 3, lens, 4, 2, 64, 16, torch.bfloat16, extra_rows=5,
                     bad_pages=[(3, 1, -1), (4, 0, 10**9), (4, 5, -2**31), (5, 2, 2**31 - 1)], width_slack=0))
     check(torch, tuple(inp), 16, max_new=max_new)
-    inp[3] = [r[:9] for r in inp[3]]  # request 4 and 5 need 13 and 10 entries
+    inp[5][3], inp[5][5] = 10**4, 2**31 - 1
     check(torch, tuple(inp), 16, max_new=max_new)
     check(torch, make(torch, 3, [(0, 0), (0, 0)], 4, 2, 64, 16, torch.bfloat16, extra_rows=2), 16, max_new=max_new)
 

@@ -41,7 +41,7 @@ struct ShLayout {
   static constexpr uint32_t bars = ml + 8 * 16 * 2 * 4;
   static constexpr uint32_t share = bars + 2 * stages * 8;
   static constexpr uint32_t part = share + 64;          // schedule scratch
-  static constexpr uint32_t smem = part + 128 + 1024;   // + alignment slack
+  static constexpr uint32_t smem = part + sizeof(PaScratch<kShThreads>) + 1024;  // + alignment slack
 };
 static_assert(sizeof(PaShare) <= 64, "the share fits its space");
 
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
     }
     fence_barrier_init();
   }
-  pa_schedule<ROWS, kShKeys, kShThreads>(p, share, reinterpret_cast<long long*>(sm + L::part));
+  pa_schedule<ROWS, kShKeys, kShThreads>(p, share, reinterpret_cast<PaScratch<kShThreads>*>(sm + L::part));
   PaWalk<ROWS, kShKeys> walk(*share);
   PaSeg sg;
   const int rows_page = min(1 << p.shift, kShKeys);  // key rows of a box
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = rg0 + g + 8 * i;
-        const int pr = sg.blk * ROWS + r, tok = pr / p.G, head = sg.h * p.G + pr - tok * p.G;
+        const int pr = sg.blk * ROWS + r, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
         const bool live = r < sg.it.rows;
         pos[i] = live ? sg.r.pos0 + tok : -1;
         src[i] = live ? p.q + (sg.r.row0 + tok) * p.q_stride + static_cast<long long>(head) * D : nullptr;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
-    const int min_pos = sg.r.pos0 + sg.blk * ROWS / p.G;  // of the block's first row
+    const int min_pos = sg.r.pos0 + pa_div_g(p, sg.blk * ROWS);  // of the block's first row
     for (int t = sg.t0; t < sg.t1; ++t, ++it) {
       if (RG == 1 && (it & 1) != half) continue;
       const int s = it % ST;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
         }
       }
       if (sg.starts && sg.ends) {
-        const int pr = sg.blk * ROWS + r, tok = pr / p.G, head = sg.h * p.G + pr - tok * p.G;
+        const int pr = sg.blk * ROWS + r, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
         const float inv = Ls > 0.f ? 1.0f / Ls : 0.f;
         uint16_t* dst = p.out + (sg.r.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + e0;
 #pragma unroll
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
                                                           pa_pack<T>(acc[e + 2] * inv, acc[e + 3] * inv));
         if (p.lse && e0 == 0)
           p.lse[static_cast<long long>(sg.r.row0 + tok) * p.hq + head] =
-              M == -INFINITY ? -INFINITY : (M + log2f(Ls)) * 0.69314718055994530942f;
+              Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * 0.69314718055994530942f;
       } else {
         const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
         float* dst = p.part_o + (slot * ROWS + r) * D + e0;
@@ -346,44 +346,54 @@ __global__ void __launch_bounds__(kShThreads, 1)
   }
 }
 
-// Adds the parts of the items that CTA blockIdx.x of the first kernel finished
-// for others: 8 output values a thread, parts in tile order.
+// Adds the parts of the item that CTA blockIdx.x of the first kernel finished
+// for others: 8 output values a thread, parts in tile order, kPaBatch of them
+// loaded at a time (one by one, nine parts took 9 us of dependent loads).
+constexpr int kPaBatch = 8;
 template <class T, int D, int ROWS>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PaParams p) {
   grid_dependency_wait();
   const PaDesc d = p.desc[blockIdx.x];
   if (!d.finish) return;
-  const int at = (blockIdx.y * 256 + threadIdx.x) * 8, r = at / D, e0 = at % D;
-  const PaReq rq = pa_request(p, d.b);
-  if (r >= min(ROWS, rq.n * p.G - d.blk * ROWS)) return;
-  // the CTA whose share holds the item's first unit
-  auto start = [&](long long j) { return d.total * j / d.active; };
-  int j0 = static_cast<int>(d.item_first * d.active / d.total);
-  while (j0 + 1 < d.active && start(j0 + 1) <= d.item_first) ++j0;
-  while (j0 > 0 && start(j0) > d.item_first) --j0;
-  const int skew = start(j0) == d.item_first ? 0 : 1;  // its part lies in its second slot unless its share starts there
+  constexpr bool kByDims = ROWS == kPaMaxRows;  // the layout of the parts
+  const int at = blockIdx.y * 256 + threadIdx.x;
+  const int r = kByDims ? at % ROWS : at / (D / 8), e0 = kByDims ? at / ROWS * 8 : at % (D / 8) * 8;
+  if (r >= d.rows) return;
   float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int j = j0; j <= static_cast<int>(blockIdx.x); ++j) {
-    const size_t slot = static_cast<size_t>(j) * 2 + (j == j0 ? skew : 0);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (slot * ROWS + r) * 2);
-    const float4 a = *reinterpret_cast<const float4*>(p.part_o + (slot * ROWS + r) * D + e0);
-    const float4 b = *reinterpret_cast<const float4*>(p.part_o + (slot * ROWS + r) * D + e0 + 4);
-    if (ml.x == -INFINITY) continue;  // no visible key among these tiles
-    const float m = fmaxf(M, ml.x), fa = ex2(M - m), fb = ex2(ml.x - m);  // M = -inf: 0
-    M = m;
-    L = L * fa + ml.y * fb;
-    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  for (int j0 = d.first; j0 <= static_cast<int>(blockIdx.x); j0 += kPaBatch) {
+    float2 ml[kPaBatch];
+    float4 a[kPaBatch], b[kPaBatch];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * fa + v[e] * fb;
+    for (int u = 0; u < kPaBatch; ++u) {
+      const int j = j0 + u;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (j <= static_cast<int>(blockIdx.x)) {
+        const size_t slot = static_cast<size_t>(j) * 2 + (j == d.first ? d.slot : 0);
+        const float4* o = reinterpret_cast<const float4*>(p.part_o) + slot * (ROWS * D / 4);
+        ml[u] = *reinterpret_cast<const float2*>(p.part_ml + (slot * ROWS + r) * 2);
+        a[u] = kByDims ? o[e0 / 4 * ROWS + r] : o[(r * D + e0) / 4];
+        b[u] = kByDims ? o[(e0 / 4 + 1) * ROWS + r] : o[(r * D + e0) / 4 + 1];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kPaBatch; ++u) {
+      if (ml[u].y == 0.f) continue;  // no such part, or no visible key among its tiles
+      const float m = fmaxf(M, ml[u].x), fa = ex2(M - m), fb = ex2(ml[u].x - m);  // M = -inf: 0
+      M = m;
+      L = L * fa + ml[u].y * fb;
+      const float v[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = acc[e] * fa + v[e] * fb;
+    }
   }
-  const int pr = d.blk * ROWS + r, tok = pr / p.G, head = d.h * p.G + pr - tok * p.G;
-  const float inv = L > 0.f ? 1.0f / L : 0.f;
-  uint16_t* dst = p.out + (rq.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + e0;
+  const int pr = d.blk * ROWS + r, tok = pa_div_g(p, pr), head = d.h * p.G + pr - tok * p.G;
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  uint16_t* dst = p.out + (d.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + e0;
   *reinterpret_cast<uint4*>(dst) = make_uint4(pa_pack<T>(acc[0] * inv, acc[1] * inv), pa_pack<T>(acc[2] * inv, acc[3] * inv),
                                               pa_pack<T>(acc[4] * inv, acc[5] * inv), pa_pack<T>(acc[6] * inv, acc[7] * inv));
   if (p.lse && e0 == 0)
-    p.lse[static_cast<long long>(rq.row0 + tok) * p.hq + head] =
-        M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.69314718055994530942f;
+    p.lse[static_cast<long long>(d.row0 + tok) * p.hq + head] =
+        L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994530942f;
 }
 
 template <class K>
@@ -469,10 +479,14 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   PaParams p{};
   p.B = static_cast<int>(a.requests), p.T = static_cast<int>(a.tokens);
   p.hq = static_cast<int>(a.q_heads), p.hk = static_cast<int>(a.kv_heads), p.G = p.hq / p.hk;
+  p.g_shift = 31;
+  while ((1 << (p.g_shift - 31)) < p.G) ++p.g_shift;
+  p.g_mul = static_cast<uint32_t>(((1ull << p.g_shift) + p.G - 1) / p.G);
   p.shift = 4;
   while ((1u << p.shift) < a.page_size) ++p.shift;
   p.pages = static_cast<int>(a.pages), p.width = static_cast<int>(a.table_width);
   p.window = static_cast<int>(a.window);
+  p.longest = static_cast<int>(std::min<uint64_t>(a.table_width * a.page_size, INT_MAX - 1024));
   constexpr double kLog2e = 1.44269504088896340736;
   p.negate = a.scale < 0.f && !(a.softcap > 0.f) && !a.alibi;
   p.scale_log2 = static_cast<float>((p.negate ? -a.scale : a.scale) * kLog2e);

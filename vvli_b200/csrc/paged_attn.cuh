@@ -31,15 +31,18 @@ constexpr int kPaMaxRows = 256;    // rows of an item at most
 
 struct PaDesc {  // what the combine kernel needs of a CTA
   int finish;    // its first segment ends an item that another CTA began
-  int b, h, blk;
-  int active;    // CTAs with a share
+  int h, blk;    // that item: kv head, block
+  int row0;      // first q row of its request
+  int rows;      // its packed rows
+  int first;     // the CTA that began it; its part is in slot `slot`, the later CTAs' in slot 0
+  int slot;
   int pad;
-  long long item_first;  // first unit of that item
-  long long total;       // units of the call
 };
 
 struct PaParams {
   int B, T, hq, hk, G, shift, pages, width;  // page_size = 1 << shift
+  int longest;                               // what a table row holds: seq_len is cut there
+  uint32_t g_mul, g_shift;                   // x / G = x * g_mul >> g_shift for 0 <= x < 2^31
   int window;                                // 0: none
   float scale_log2;                          // scale * log2(e); its magnitude without a feature, then
   int negate;                                // the sign goes into q
@@ -54,7 +57,7 @@ struct PaParams {
   int* err;
   PaDesc* desc;    // [kPaMaxCtas]
   float* part_ml;  // [kPaMaxCtas][2][kPaMaxRows][2] running maximum (log2 units) and sum
-  float* part_o;   // [kPaMaxCtas][2][rows of an item][D]
+  float* part_o;   // [kPaMaxCtas][2] sums of an item's rows: [rows][D], or [D / 4][rows][4] (256 rows, a thread each)
 };
 
 inline size_t pa_workspace_bytes(int d) {
@@ -83,9 +86,17 @@ VVLI_DEV PaReq pa_request(const PaParams& p, int b) {
   PaReq r;
   r.row0 = c0;
   r.n = min(c1, p.T) - c0;
-  // lengths that no cache holds are cut, so that positions and tiles stay in 32 bits
-  r.pos0 = max(min(p.seq[b], INT_MAX - 1024), 0) - (c1 - c0);
+  r.pos0 = max(min(p.seq[b], p.longest), 0) - (c1 - c0);
   return r;
+}
+
+// g_mul = ceil(2^g_shift / G), g_shift = 31 + ceil(log2 G): exact, since x * (g_mul G - 2^g_shift) < 2^g_shift.
+VVLI_DEV int pa_div_g(const PaParams& p, int x) {
+  return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * p.g_mul >> p.g_shift);
+}
+// a / b of small or large counts.
+VVLI_DEV long long pa_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
 template <int ROWS>
@@ -103,7 +114,7 @@ template <int ROWS, int KT>
 VVLI_DEV PaItem pa_item(const PaParams& p, const PaReq& r, int blk) {
   PaItem it;
   it.rows = min(ROWS, r.n * p.G - blk * ROWS);
-  const int first = r.pos0 + blk * ROWS / p.G, last = r.pos0 + (blk * ROWS + it.rows - 1) / p.G;
+  const int first = r.pos0 + pa_div_g(p, blk * ROWS), last = r.pos0 + pa_div_g(p, blk * ROWS + it.rows - 1);
   it.hi = max(0, last + 1);
   it.lo = p.window && first >= p.window ? first + 1 - p.window : 0;
   it.t0 = it.lo / KT;
@@ -112,7 +123,8 @@ VVLI_DEV PaItem pa_item(const PaParams& p, const PaReq& r, int blk) {
 }
 
 struct PaShare {
-  long long total, u0, u1;  // units of the call; this CTA's
+  long long each, more;     // units of a CTA; the first `more` CTAs have one more
+  long long u0, u1;         // this CTA's
   int active;               // CTAs with a share
   int b, h, blk, off;       // where u0 lies: item and tile of it
   long long item_first;     // first unit of that item
@@ -148,13 +160,13 @@ VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
   int nb = 0;
   if (live) r = pa_request(p, b), nb = pa_blocks<ROWS>(p, r);
   long long u = 0;
-  if (nb <= 8) {
+  if (nb <= 2) {
     for (int i = 0; i < nb; ++i) {
       const PaItem it = pa_item<ROWS, KT>(p, r, i);
       u += it.t1 - it.t0;
     }
   }
-  unsigned big = __ballot_sync(0xffffffffu, nb > 8);
+  unsigned big = __ballot_sync(0xffffffffu, nb > 2);
   while (big) {
     const int src = __ffs(big) - 1;
     big &= big - 1;
@@ -173,43 +185,51 @@ VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
   return u;
 }
 
+VVLI_DEV long long pa_start(const PaShare& s, long long i) { return s.each * i + min(i, s.more); }
+
+template <int NT>
+struct PaScratch {
+  long long part[NT / 32];
+  long long units[NT];  // of one kv head of each request
+};
+
+// Units of requests b0 .. b0 + NT: thread t gets request b0 + t's, those of one
+// head, and the units of all heads of the requests before it.  Neighbouring
+// requests go to different warps, which share the ones of many blocks.
+template <int ROWS, int KT, int NT>
+VVLI_DEV long long pa_count(const PaParams& p, int b0, PaScratch<NT>* sc, long long& units, long long& before) {
+  const int at = (threadIdx.x & 31) * (NT / 32) + (threadIdx.x >> 5);
+  __syncthreads();
+  sc->units[at] = pa_units<ROWS, KT>(p, b0 + at, b0 + at < p.B);
+  __syncthreads();
+  units = sc->units[threadIdx.x];
+  long long total;
+  before = pa_scan<NT>(units * p.hk, sc->part, total);
+  return total;
+}
+
 // This CTA's share, worked out by all its NT threads; valid in `out` (shared) after the call.
 template <int ROWS, int KT, int NT>
-VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, long long* part) {
+VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, PaScratch<NT>* sc) {
   const int tid = threadIdx.x;
-  long long total = 0, t, first_units = 0, first_before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += NT) {
-    const int b = b0 + tid;
-    const long long u = pa_units<ROWS, KT>(p, b, b < p.B) * p.hk;
-    const long long before = pa_scan<NT>(u, part, t);
-    if (b0 == 0) first_units = u, first_before = before;
-    total += t;
-  }
-  const long long grid = gridDim.x;
-  const int active = static_cast<int>(min(grid, total));
-  const long long i = blockIdx.x;
-  const long long u0 = i < active ? total * i / active : 0, u1 = i < active ? total * (i + 1) / active : 0;
-  if (tid == 0) {
-    out->total = total, out->active = active, out->u0 = u0, out->u1 = u1;
-    out->b = p.B;
-  }
-  __syncthreads();
+  long long total = 0, before, units;
+  for (int b0 = 0; b0 < p.B; b0 += NT) total += pa_count<ROWS, KT, NT>(p, b0, sc, units, before);
+  const int active = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  PaShare s;
+  s.each = active ? pa_div(total, active) : 0, s.more = total - s.each * active;
+  s.active = active;
+  const bool idle = static_cast<int>(blockIdx.x) >= active;
+  const long long u0 = idle ? 0 : pa_start(s, blockIdx.x), u1 = idle ? 0 : pa_start(s, blockIdx.x + 1);
+  if (tid == 0) out->each = s.each, out->more = s.more, out->active = active, out->u0 = u0, out->u1 = u1;
   long long done = 0;
   for (int b0 = 0; b0 < p.B && u0 < u1; b0 += NT) {
-    const int b = b0 + tid;
-    long long u = first_units, before = first_before;
-    if (p.B > NT) {  // more requests than threads: the sums again
-      u = pa_units<ROWS, KT>(p, b, b < p.B) * p.hk;
-      before = pa_scan<NT>(u, part, t);
-    } else {
-      t = total;
-    }
-    before += done;
-    if (u > 0 && before <= u0 && u0 < before + u) {
-      const long long per = u / p.hk;
-      out->b = b;
-      out->h = static_cast<int>((u0 - before) / per);
-      out->item_first = before + out->h * per;  // first unit of the head, for now
+    long long t = total;
+    if (p.B > NT) t = pa_count<ROWS, KT, NT>(p, b0, sc, units, before);  // more requests than threads: again
+    const long long lead = done + before;
+    if (units > 0 && lead <= u0 && u0 < lead + units * p.hk) {
+      out->b = b0 + tid;
+      out->h = static_cast<int>(pa_div(u0 - lead, units));
+      out->item_first = lead + out->h * units;  // first unit of the head, for now
     }
     done += t;
     if (done > u0) break;  // uniform
@@ -295,12 +315,15 @@ struct PaWalk {
 VVLI_DEV int pa_slot(const PaSeg& s) { return s.at_start ? 0 : 1; }
 
 // Called by one thread per CTA: what the combine kernel does for it.
-VVLI_DEV void pa_describe(const PaParams& p, const PaShare& sh, const PaSeg* first) {
-  PaDesc d;
-  d.finish = first && !first->starts && first->ends;
-  d.b = d.finish ? first->b : 0, d.h = d.finish ? first->h : 0, d.blk = d.finish ? first->blk : 0;
-  d.item_first = d.finish ? first->item_first : 0;
-  d.active = sh.active, d.total = sh.total, d.pad = 0;
+VVLI_DEV void pa_describe(const PaParams& p, const PaShare& sh, const PaSeg* s) {
+  PaDesc d{};
+  if (s && !s->starts && s->ends) {
+    const long long wide = sh.more * (sh.each + 1);
+    const long long j = s->item_first < wide ? pa_div(s->item_first, sh.each + 1)
+                                             : sh.more + pa_div(s->item_first - wide, sh.each);
+    d.finish = 1, d.h = s->h, d.blk = s->blk, d.row0 = s->r.row0, d.rows = s->it.rows;
+    d.first = static_cast<int>(j), d.slot = pa_start(sh, j) == s->item_first ? 0 : 1;  // its second slot unless its share starts there
+  }
   p.desc[blockIdx.x] = d;
 }
 

@@ -48,7 +48,7 @@ struct TcaLayout {
   static constexpr uint32_t bars = ring + stages * kv;
   static constexpr uint32_t share = bars + 320;        // 3 stages + 11 barriers and the TMEM address
   static constexpr uint32_t part = share + 64;
-  static constexpr uint32_t smem = part + 128 + 1024;  // + alignment slack
+  static constexpr uint32_t smem = part + sizeof(PaScratch<kTcThreads>) + 1024;  // + alignment slack
   static constexpr uint32_t o_col = 256;               // S_0 at column 0, S_1 at 128, O_t at 256 + D t
   static constexpr uint32_t slice = 128 * 128;         // bytes of a 64-element slice of a 128-row tile
 };
@@ -205,7 +205,7 @@ VVLI_DEV void tca_cap(const PaParams& p, float* s) {
 VVLI_DEV int tca_tiles(const PaParams& p, const PaSeg& s, int t) {
   const int rows = min(kTcTile, s.it.rows - t * kTcTile);
   if (rows <= 0) return 0;
-  const int last = s.r.pos0 + (s.blk * kTcRows + t * kTcTile + rows - 1) / p.G;
+  const int last = s.r.pos0 + pa_div_g(p, s.blk * kTcRows + t * kTcTile + rows - 1);
   const int end = max(s.it.t0 + 1, (max(0, last + 1) + kTcKeys - 1) / kTcKeys);
   return max(0, min(s.t1, end) - s.t0);
 }
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  pa_schedule<kTcRows, kTcKeys, kTcThreads>(p, share, reinterpret_cast<long long*>(sm + L::part));  // has barriers
+  pa_schedule<kTcRows, kTcKeys, kTcThreads>(p, share, reinterpret_cast<PaScratch<kTcThreads>*>(sm + L::part));  // has barriers
   tc_fence_after();
   const uint32_t tmem = *holder;
   PaWalk<kTcRows, kTcKeys> walk(*share);
@@ -393,7 +393,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int t = warp >> 2, R = kTcTile * t + 32 * (warp & 3) + lane;  // row of the item
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + L::o_col + t * D;
-    uint8_t* qrow = sm + t * L::q_tile + (R & 127) * 128;
     uint32_t ss = 0, os = 0;  // waits on s_full, o_full so far
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-wide: what follows is
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
@@ -401,24 +400,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     while (!dead && walk.next(p, sg)) {
       const int nt = tca_tiles(p, sg, t);
-      const int pr = sg.blk * kTcRows + R, tok = pr / p.G, head = sg.h * p.G + pr - tok * p.G;
+      const int pr = sg.blk * kTcRows + R, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
       const bool live = R < sg.it.rows;
       const int pos = live ? sg.r.pos0 + tok : -1;
-      const int first_pos = sg.r.pos0 + (sg.blk * kTcRows + t * kTcTile) / p.G;  // of this tile's first row
+      const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows + t * kTcTile);  // of this tile's first row
       const int last_pos = sg.it.hi - 1;
       float m = -INFINITY, l = 0.f;
       const float slope = (FEAT & kPaAlibi) && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
       if (nt > 0) {
-        const uint16_t* src = p.q + (sg.r.row0 + tok) * p.q_stride + static_cast<long long>(head) * D;
+        // D / 8 lanes side by side read a row: 16-byte chunk c of rows i * (256 / D) + lane / (D / 8) of the warp's 32
+        const uint32_t sign = p.negate ? 0x80008000u : 0u;
+        const int c = lane % (D / 8), w0 = 32 * (warp & 3), pr0 = sg.blk * kTcRows + t * kTcTile + w0;
+        uint8_t* dst = sm + t * L::q_tile + (c >> 3) * L::slice;
         uint4 v[D / 8];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          v[c] = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < D / 8; ++i) {
+          const int row = i * (256 / D) + lane / (D / 8), rp = pr0 + row, rt = pa_div_g(p, rp);
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (t * kTcTile + w0 + row < sg.it.rows)
+            v[i] = *reinterpret_cast<const uint4*>(p.q + (sg.r.row0 + rt) * p.q_stride +
+                                                   static_cast<long long>(sg.h * p.G + rp - rt * p.G) * D + 8 * c);
         }
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          if (p.negate) v[c].x ^= 0x80008000u, v[c].y ^= 0x80008000u, v[c].z ^= 0x80008000u, v[c].w ^= 0x80008000u;
-          *reinterpret_cast<uint4*>(qrow + (c >> 3) * L::slice + (((c & 7) ^ (R & 7)) << 4)) = v[c];
+        for (int i = 0; i < D / 8; ++i) {
+          const int row = w0 + i * (256 / D) + lane / (D / 8);
+          *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+              make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
         }
         tca_fence_async();
         mbar_arrive(&q_full[t]);
@@ -506,19 +513,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (dead) break;
       const bool whole = sg.starts && sg.ends;
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
-      const float inv = m == -INFINITY && l == l ? 0.f : 1.0f / l;  // no visible key: zeros; NaN stays
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // no visible key: zeros
       if (live) {
         if (whole) {
           if (p.lse)
             p.lse[static_cast<long long>(sg.r.row0 + tok) * p.hq + head] =
-                m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
         } else {
           *reinterpret_cast<float2*>(p.part_ml + (slot * kTcRows + R) * 2) = make_float2(m, l);
         }
       }
       if (nt > 0) {
         uint16_t* dst = p.out + (sg.r.row0 + tok) * p.out_stride + static_cast<long long>(head) * D;
-        float* part = p.part_o + (slot * kTcRows + R) * D;
+        float4* part = reinterpret_cast<float4*>(p.part_o) + slot * (kTcRows * D / 4) + R;  // four dims of all rows together
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              part[(32 * c + i) / 4 * kTcRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
       }
