@@ -138,6 +138,7 @@ def test_empty_rows_bad_pages_and_rows_behind(torch, max_new):
     inp = list(make(torch, 3, lens, 4, 2, 64, 16, torch.bfloat16, extra_rows=5,
                     bad_pages=[(3, 1, -1), (4, 0, 10**9), (4, 5, -2**31), (5, 2, 2**31 - 1)], width_slack=0))
     check(torch, tuple(inp), 16, max_new=max_new)
+    inp = list(make(torch, 3, lens, 4, 2, 64, 16, torch.bfloat16, poison=False, bad_pages=[(3, 1, -1)], width_slack=0))
     inp[5][3], inp[5][5] = 10**4, 2**31 - 1
     check(torch, tuple(inp), 16, max_new=max_new)
     check(torch, make(torch, 3, [(0, 0), (0, 0)], 4, 2, 64, 16, torch.bfloat16, extra_rows=2), 16, max_new=max_new)

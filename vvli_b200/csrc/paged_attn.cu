@@ -347,53 +347,75 @@ __global__ void __launch_bounds__(kShThreads, 1)
 }
 
 // Adds the parts of the item that CTA blockIdx.x of the first kernel finished
-// for others: 8 output values a thread, parts in tile order, kPaBatch of them
-// loaded at a time (one by one, nine parts took 9 us of dependent loads).
-constexpr int kPaBatch = 8;
-template <class T, int D, int ROWS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const PaParams p) {
-  grid_dependency_wait();
-  const PaDesc d = p.desc[blockIdx.x];
-  if (!d.finish) return;
-  constexpr bool kByDims = ROWS == kPaMaxRows;  // the layout of the parts
-  const int at = blockIdx.y * 256 + threadIdx.x;
-  const int r = kByDims ? at % ROWS : at / (D / 8), e0 = kByDims ? at / ROWS * 8 : at % (D / 8) * 8;
-  if (r >= d.rows) return;
-  float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int j0 = d.first; j0 <= static_cast<int>(blockIdx.x); j0 += kPaBatch) {
-    float2 ml[kPaBatch];
-    float4 a[kPaBatch], b[kPaBatch];
+// for others, in tile order; 4 or 8 output values a thread.
+template <int N, int F4>
+struct CombineState {
+  float M = -INFINITY, L = 0.f;
+  float4 acc[F4] = {};
+  // Parts j0 .. j0 + N (past `last`: the last again, with no weight), loaded
+  // together: one by one, nine parts took 9 us of dependent loads.
+  VVLI_DEV void add(const float2* mls, const float4* parts, const PaDesc& d, int j0, int last, int rows, size_t floats4,
+                    int apart) {
+    float2 ml[N];
+    float4 v[N][F4];
 #pragma unroll
-    for (int u = 0; u < kPaBatch; ++u) {
-      const int j = j0 + u;
-      ml[u] = make_float2(-INFINITY, 0.f);
-      if (j <= static_cast<int>(blockIdx.x)) {
-        const size_t slot = static_cast<size_t>(j) * 2 + (j == d.first ? d.slot : 0);
-        const float4* o = reinterpret_cast<const float4*>(p.part_o) + slot * (ROWS * D / 4);
-        ml[u] = *reinterpret_cast<const float2*>(p.part_ml + (slot * ROWS + r) * 2);
-        a[u] = kByDims ? o[e0 / 4 * ROWS + r] : o[(r * D + e0) / 4];
-        b[u] = kByDims ? o[(e0 / 4 + 1) * ROWS + r] : o[(r * D + e0) / 4 + 1];
-      }
+    for (int u = 0; u < N; ++u) {
+      const int j = min(j0 + u, last);
+      const size_t slot = static_cast<size_t>(j) * 2 + (j == d.first ? d.slot : 0);
+      ml[u] = mls[slot * rows];
+#pragma unroll
+      for (int f = 0; f < F4; ++f) v[u][f] = parts[slot * floats4 + f * apart];
+      if (j0 + u > last) ml[u].y = 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < kPaBatch; ++u) {
+    for (int u = 0; u < N; ++u) {
       if (ml[u].y == 0.f) continue;  // no such part, or no visible key among its tiles
       const float m = fmaxf(M, ml[u].x), fa = ex2(M - m), fb = ex2(ml[u].x - m);  // M = -inf: 0
       M = m;
       L = L * fa + ml[u].y * fb;
-      const float v[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = acc[e] * fa + v[e] * fb;
+      for (int f = 0; f < F4; ++f) {
+        acc[f].x = acc[f].x * fa + v[u][f].x * fb, acc[f].y = acc[f].y * fa + v[u][f].y * fb;
+        acc[f].z = acc[f].z * fa + v[u][f].z * fb, acc[f].w = acc[f].w * fa + v[u][f].w * fb;
+      }
     }
   }
+};
+
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(256, ROWS == kPaMaxRows ? 4 : 2) paged_combine_kernel(const PaParams p) {
+  grid_dependency_wait();
+  const PaDesc d = p.desc[blockIdx.x];
+  if (!d.finish) return;
+  constexpr bool kByDims = ROWS == kPaMaxRows;  // the layout of the parts
+  constexpr int F4 = kByDims ? 2 : 1;           // float4s of a thread
+  const int at = blockIdx.y * 256 + threadIdx.x;
+  // by dims: four threads side by side have 32 dims of a row, so that reads and writes are runs of 64 bytes or more
+  const int r = kByDims ? at / 4 % ROWS : at / (D / 4);
+  const int e4 = kByDims ? (at % 4 + at / (4 * ROWS) * 4) * 2 : at % (D / 4);
+  if (r >= d.rows) return;
+  const float4* parts = reinterpret_cast<const float4*>(p.part_o) + (kByDims ? e4 * ROWS + r : r * (D / 4) + e4);
+  const float2* mls = reinterpret_cast<const float2*>(p.part_ml) + r;
+  const int last = blockIdx.x;
+  constexpr int N = kByDims ? 4 : 8;  // a chunk's item has two or three parts, a lone decode token one per CTA
+  CombineState<N, F4> s;
+  for (int j0 = d.first; j0 <= last; j0 += N) s.add(mls, parts, d, j0, last, ROWS, ROWS * D / 4, ROWS);
   const int pr = d.blk * ROWS + r, tok = pa_div_g(p, pr), head = d.h * p.G + pr - tok * p.G;
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  uint16_t* dst = p.out + (d.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + e0;
-  *reinterpret_cast<uint4*>(dst) = make_uint4(pa_pack<T>(acc[0] * inv, acc[1] * inv), pa_pack<T>(acc[2] * inv, acc[3] * inv),
-                                              pa_pack<T>(acc[4] * inv, acc[5] * inv), pa_pack<T>(acc[6] * inv, acc[7] * inv));
-  if (p.lse && e0 == 0)
+  const float inv = s.L == 0.f ? 0.f : 1.0f / s.L;
+  uint16_t* dst = p.out + (d.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + 4 * e4;
+  uint32_t o[2 * F4];
+#pragma unroll
+  for (int f = 0; f < F4; ++f) {
+    o[2 * f] = pa_pack<T>(s.acc[f].x * inv, s.acc[f].y * inv);
+    o[2 * f + 1] = pa_pack<T>(s.acc[f].z * inv, s.acc[f].w * inv);
+  }
+  if constexpr (kByDims)
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  else
+    *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+  if (p.lse && e4 == 0)
     p.lse[static_cast<long long>(d.row0 + tok) * p.hq + head] =
-        L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994530942f;
+        s.L == 0.f ? -INFINITY : (s.M + log2f(s.L)) * 0.69314718055994530942f;
 }
 
 template <class K>
@@ -521,7 +543,7 @@ cudaError_t pa_queue_combine(const PaParams& p, int ctas, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), (ROWS * D + 2047) / 2048);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), ROWS == kPaMaxRows ? D / 8 : (ROWS * D / 4 + 255) / 256);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cfg.attrs = attr;

@@ -19,6 +19,8 @@
 //   * MMAs are issued in the order P_0 V_j, S_0 of j + 1, P_1 V_j, S_1 of
 //     j + 1; they run in that order, so S of a tile may overwrite the P before
 //     it, and a softmax thread that sees S of j + 1 knows P V of j is done.
+//   * An item of at most 128 rows is worked on by both tiles, alternate key tiles
+//     each.
 //   * Warps 0-3 and 4-7: softmax of tile 0 and 1, loading Q and writing the
 //     output; warp 8 issues the MMAs, warp 9 the copies, warp 10 clears the
 //     values past the last visible key in shared memory (they may be anything,
@@ -201,8 +203,21 @@ VVLI_DEV void tca_cap(const PaParams& p, float* s) {
   }
 }
 
-// Tiles of this segment that row tile t works on (its rows see no later key).
+// An item of at most 128 rows would leave one row tile idle and the other
+// waiting for its own MMAs: both tiles then hold the same rows and take the key
+// tiles in turn (twins), and tile 1's sums are added to tile 0's at the end.
+// That reads two tiles ahead, which the ring's four stages at head_dim 128 do not
+// reach: 16 requests of 16,000 keys and 48 rows took 114 us against 164 at
+// head_dim 64, but 268 against 197 at 128.
+template <int D>
+VVLI_DEV bool tca_twins(const PaSeg& s) {
+  return D == 64 && s.it.rows <= kTcTile;
+}
+
+// Key tiles of this segment that row tile t works on (its rows see no later key).
+template <int D>
 VVLI_DEV int tca_tiles(const PaParams& p, const PaSeg& s, int t) {
+  if (tca_twins<D>(s)) return (s.t1 - s.t0 + 1 - t) >> 1;
   const int rows = min(kTcTile, s.it.rows - t * kTcTile);
   if (rows <= 0) return 0;
   const int last = s.r.pos0 + pa_div_g(p, s.blk * kTcRows + t * kTcTile + rows - 1);
@@ -358,7 +373,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!dead && j + 1 < nt) issue_s(t, ks);
       };
       while (!dead && walk.next(p, sg)) {
-        const int N = sg.t1 - sg.t0, nt0 = tca_tiles(p, sg, 0), nt1 = tca_tiles(p, sg, 1);
+        const int N = sg.t1 - sg.t0;
+        if (tca_twins<D>(sg)) {
+          for (int j = 0; j < min(N, 2) && !dead; ++j) {
+            const uint32_t k = n + 2 * j;
+            wait(&full[k % ST], k / ST);
+            wait(&q_full[j], j ? q_par1 : q_par0);
+            if (dead) break;
+            issue_s(j, k % ST);
+            tca_commit(&empty[k % ST]);
+          }
+          q_par0 ^= 1;
+          if (N > 1) q_par1 ^= 1;
+          for (int j = 0; j < N && !dead; ++j) {
+            const int t = j & 1;
+            const uint32_t v = n + 2 * j + 1, k = v + 3, par = t ? p_par1 : p_par0;
+            wait(&v_ready[v % ST], v / ST);
+            if (j + 2 < N) wait(&full[k % ST], k / ST);
+            wait(&p_half[t], par);
+            tc_fence_after();
+            if (!dead) issue_pv(t, v % ST, 0, j >> 1);
+            wait(&p_full[t], par);
+            tc_fence_after();
+            if (dead) break;
+            issue_pv(t, v % ST, 1, j >> 1);
+            if (t)
+              p_par1 ^= 1;
+            else
+              p_par0 ^= 1;
+            if (j + 2 >= N) tca_commit(&o_full[t]);
+            if (j + 2 < N) {
+              issue_s(t, k % ST);
+              tca_commit(&empty[k % ST]);
+            }
+            tca_commit(&empty[v % ST]);
+          }
+          n += 2 * N;
+          continue;
+        }
+        const int nt0 = tca_tiles<D>(p, sg, 0), nt1 = tca_tiles<D>(p, sg, 1);
         wait(&full[n % ST], n / ST);
         if (nt0) {
           wait(&q_full[0], q_par0);
@@ -390,34 +443,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax of row tile t: thread = row
-    const int t = warp >> 2, R = kTcTile * t + 32 * (warp & 3) + lane;  // row of the item
+    const int t = warp >> 2, lane_row = 32 * (warp & 3) + lane;  // TMEM lane
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + L::o_col + t * D;
+    // where twins' tile 1 leaves its sums: O over both tiles' q, [D / 4][128][4], and (m, l) over the schedule's scratch
+    float4* twin_o = reinterpret_cast<float4*>(sm) + lane_row;
+    float2* twin_ml = reinterpret_cast<float2*>(sm + L::part) + lane_row;
     uint32_t ss = 0, os = 0;  // waits on s_full, o_full so far
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-wide: what follows is
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
       tc_fence_after();
     };
-    while (!dead && walk.next(p, sg)) {
-      const int nt = tca_tiles(p, sg, t);
+    while (walk.next(p, sg)) {  // after a wait gave up too: the tiles' barriers below need all threads
+      const int nt = tca_tiles<D>(p, sg, t);
+      const bool twins = tca_twins<D>(sg);
+      const int row0 = twins ? 0 : t * kTcTile, R = row0 + lane_row;  // row of the item
       const int pr = sg.blk * kTcRows + R, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
       const bool live = R < sg.it.rows;
       const int pos = live ? sg.r.pos0 + tok : -1;
-      const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows + t * kTcTile);  // of this tile's first row
+      const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows + row0);  // of this tile's first row
       const int last_pos = sg.it.hi - 1;
       float m = -INFINITY, l = 0.f;
       const float slope = (FEAT & kPaAlibi) && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
-      if (nt > 0) {
+      if (nt > 0 && !dead) {
         // D / 8 lanes side by side read a row: 16-byte chunk c of rows i * (256 / D) + lane / (D / 8) of the warp's 32
         const uint32_t sign = p.negate ? 0x80008000u : 0u;
-        const int c = lane % (D / 8), w0 = 32 * (warp & 3), pr0 = sg.blk * kTcRows + t * kTcTile + w0;
+        const int c = lane % (D / 8), w0 = 32 * (warp & 3), pr0 = sg.blk * kTcRows + row0 + w0;
         uint8_t* dst = sm + t * L::q_tile + (c >> 3) * L::slice;
         uint4 v[D / 8];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const int row = i * (256 / D) + lane / (D / 8), rp = pr0 + row, rt = pa_div_g(p, rp);
           v[i] = make_uint4(0, 0, 0, 0);
-          if (t * kTcTile + w0 + row < sg.it.rows)
+          if (row0 + w0 + row < sg.it.rows)
             v[i] = *reinterpret_cast<const uint4*>(p.q + (sg.r.row0 + rt) * p.q_stride +
                                                    static_cast<long long>(sg.h * p.G + rp - rt * p.G) * D + 8 * c);
         }
@@ -439,7 +497,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tca_ld_done();
 #pragma unroll
         for (int c = 0; c < 4; ++c) tca_pin(s + 32 * c);
-        const int key0 = (sg.t0 + j) * kTcKeys;
+        const int key0 = (sg.t0 + (twins ? 2 * j + t : j)) * kTcKeys;
         const int lim = pos - key0;  // columns up to here are visible
         if constexpr (FEAT & kPaCap) tca_cap(p, s);
         if constexpr (FEAT & kPaAlibi) {
@@ -508,13 +566,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
-      if (dead) break;
-      if (nt > 0) wait(&o_full[t], os++);
-      if (dead) break;
-      const bool whole = sg.starts && sg.ends;
+      if (nt > 0 && !dead) wait(&o_full[t], os++);
+      float fold = 0.f, other = 0.f;  // twins: factors of this tile's and the other's sums
+      if (twins && sg.t1 - sg.t0 > 1) {
+        named_barrier(1, 2 * kTcTile);  // both tiles' MMAs are done: q is free
+        if (t == 1) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tca_ld32(to + 32 * c, o);
+            tca_ld_done();
+            tca_pin(o);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              twin_o[(32 * c + i) / 4 * kTcTile] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          *twin_ml = make_float2(m, l);
+        }
+        named_barrier(1, 2 * kTcTile);
+        if (t == 0) {
+          const float2 ml = *twin_ml;
+          const float both = fmaxf(m, ml.x), mu = both == -INFINITY ? 0.f : both;
+          fold = ex2(m - mu), other = ex2(ml.x - mu);
+          m = both;
+          l = l * fold + ml.y * other;
+        }
+      }
+      const bool whole = sg.starts && sg.ends, mine = !dead && !(twins && t == 1);
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
       const float inv = l == 0.f ? 0.f : 1.0f / l;  // no visible key: zeros
-      if (live) {
+      if (live && mine) {
         if (whole) {
           if (p.lse)
             p.lse[static_cast<long long>(sg.r.row0 + tok) * p.hq + head] =
@@ -523,7 +604,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           *reinterpret_cast<float2*>(p.part_ml + (slot * kTcRows + R) * 2) = make_float2(m, l);
         }
       }
-      if (nt > 0) {
+      if (nt > 0 && mine) {
         uint16_t* dst = p.out + (sg.r.row0 + tok) * p.out_stride + static_cast<long long>(head) * D;
         float4* part = reinterpret_cast<float4*>(p.part_o) + slot * (kTcRows * D / 4) + R;  // four dims of all rows together
 #pragma unroll 1
@@ -533,6 +614,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tca_ld_done();
           tca_pin(o);
           if (!live) continue;  // the loads are warp-wide
+          if (other != 0.f || fold != 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 v = twin_o[(32 * c + i) / 4 * kTcTile];
+              o[i] = o[i] * fold + v.x * other, o[i + 1] = o[i + 1] * fold + v.y * other;
+              o[i + 2] = o[i + 2] * fold + v.z * other, o[i + 3] = o[i + 3] * fold + v.w * other;
+            }
+          }
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
@@ -546,6 +635,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
+      if (twins && sg.t1 - sg.t0 > 1) named_barrier(1, 2 * kTcTile);  // tile 1's sums are read before q is written again
     }
   }
   tc_fence_before();
