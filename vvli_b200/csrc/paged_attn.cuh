@@ -3,8 +3,9 @@
 //
 // Work.  A request's query rows of one kv head are packed: row r is the new
 // token r / G and the group's q head r % G.  An item is (request, kv head,
-// block of ROWS packed rows); its units are the KT-key tiles that any of its
-// rows sees.  The units of all items in order (request, head, block, tile)
+// block of ROWS packed rows); it counts the KT-key tiles that any of its rows
+// sees, and EXTRA units more, which stand for its start and end (q in, sums
+// out) and come first.  The units of all items in order (request, head, block, tile)
 // form one line that is cut into equal shares, one per CTA, whatever the
 // lengths: a CTA's share is a run of segments, each a range of one item's
 // tiles.  A segment that is a whole item writes its output; the others (at most
@@ -126,7 +127,7 @@ struct PaShare {
   long long each, more;     // units of a CTA; the first `more` CTAs have one more
   long long u0, u1;         // this CTA's
   int active;               // CTAs with a share
-  int b, h, blk, off;       // where u0 lies: item and tile of it
+  int b, h, blk, off;       // where u0 lies: item and unit of it
   long long item_first;     // first unit of that item
 };
 
@@ -153,8 +154,8 @@ VVLI_DEV long long pa_scan(long long v, long long* part, long long& total) {
   return before + s - v;
 }
 
-// Tiles of one kv head of request b over all its blocks; a warp works out requests of many blocks together.
-template <int ROWS, int KT>
+// Units of one kv head of request b over all its blocks; a warp works out requests of many blocks together.
+template <int ROWS, int KT, int EXTRA>
 VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
   PaReq r{0, 0, 0};
   int nb = 0;
@@ -163,7 +164,7 @@ VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
   if (nb <= 2) {
     for (int i = 0; i < nb; ++i) {
       const PaItem it = pa_item<ROWS, KT>(p, r, i);
-      u += it.t1 - it.t0;
+      u += it.t1 - it.t0 + EXTRA;
     }
   }
   unsigned big = __ballot_sync(0xffffffffu, nb > 2);
@@ -176,7 +177,7 @@ VVLI_DEV long long pa_units(const PaParams& p, int b, bool live) {
     long long s = 0;
     for (int i = threadIdx.x & 31; i < n; i += 32) {
       const PaItem it = pa_item<ROWS, KT>(p, o, i);
-      s += it.t1 - it.t0;
+      s += it.t1 - it.t0 + EXTRA;
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -196,11 +197,11 @@ struct PaScratch {
 // Units of requests b0 .. b0 + NT: thread t gets request b0 + t's, those of one
 // head, and the units of all heads of the requests before it.  Neighbouring
 // requests go to different warps, which share the ones of many blocks.
-template <int ROWS, int KT, int NT>
+template <int ROWS, int KT, int EXTRA, int NT>
 VVLI_DEV long long pa_count(const PaParams& p, int b0, PaScratch<NT>* sc, long long& units, long long& before) {
   const int at = (threadIdx.x & 31) * (NT / 32) + (threadIdx.x >> 5);
   __syncthreads();
-  sc->units[at] = pa_units<ROWS, KT>(p, b0 + at, b0 + at < p.B);
+  sc->units[at] = pa_units<ROWS, KT, EXTRA>(p, b0 + at, b0 + at < p.B);
   __syncthreads();
   units = sc->units[threadIdx.x];
   long long total;
@@ -209,11 +210,11 @@ VVLI_DEV long long pa_count(const PaParams& p, int b0, PaScratch<NT>* sc, long l
 }
 
 // This CTA's share, worked out by all its NT threads; valid in `out` (shared) after the call.
-template <int ROWS, int KT, int NT>
+template <int ROWS, int KT, int EXTRA, int NT>
 VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, PaScratch<NT>* sc) {
   const int tid = threadIdx.x;
   long long total = 0, before, units;
-  for (int b0 = 0; b0 < p.B; b0 += NT) total += pa_count<ROWS, KT, NT>(p, b0, sc, units, before);
+  for (int b0 = 0; b0 < p.B; b0 += NT) total += pa_count<ROWS, KT, EXTRA, NT>(p, b0, sc, units, before);
   const int active = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   PaShare s;
   s.each = active ? pa_div(total, active) : 0, s.more = total - s.each * active;
@@ -224,7 +225,7 @@ VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, PaScratch<NT>* sc) {
   long long done = 0;
   for (int b0 = 0; b0 < p.B && u0 < u1; b0 += NT) {
     long long t = total;
-    if (p.B > NT) t = pa_count<ROWS, KT, NT>(p, b0, sc, units, before);  // more requests than threads: again
+    if (p.B > NT) t = pa_count<ROWS, KT, EXTRA, NT>(p, b0, sc, units, before);  // more requests than threads: again
     const long long lead = done + before;
     if (units > 0 && lead <= u0 && u0 < lead + units * p.hk) {
       out->b = b0 + tid;
@@ -244,7 +245,7 @@ VVLI_DEV void pa_schedule(const PaParams& p, PaShare* out, PaScratch<NT>* sc) {
       int n = 0;
       if (k < nb) {
         const PaItem it = pa_item<ROWS, KT>(p, r, k);
-        n = it.t1 - it.t0;
+        n = it.t1 - it.t0 + EXTRA;
       }
       long long s = n;
 #pragma unroll
@@ -274,7 +275,7 @@ struct PaSeg {
   long long item_first;
 };
 
-template <int ROWS, int KT>
+template <int ROWS, int KT, int EXTRA>
 struct PaWalk {
   long long u, u1, item_first;
   int b, h, blk, off;
@@ -289,16 +290,17 @@ struct PaWalk {
     s.it = pa_item<ROWS, KT>(p, s.r, blk);
     s.item_first = item_first;
     s.at_start = first;
-    s.starts = off == 0;
-    const int left = s.it.t1 - s.it.t0 - off;
+    const int left = s.it.t1 - s.it.t0 + EXTRA - off;
     const int n = static_cast<int>(min(static_cast<long long>(left), u1 - u));
-    s.t0 = s.it.t0 + off;
-    s.t1 = s.t0 + n;
+    s.t0 = s.it.t0 + max(0, off - EXTRA);
+    s.t1 = s.it.t0 + max(0, off + n - EXTRA);
+    if (s.t1 == s.t0) return false;  // the share ends before the item's first tile
+    s.starts = s.t0 == s.it.t0;
     s.ends = n == left;
     first = false;
     u += n;
     if (s.ends) {
-      item_first += s.it.t1 - s.it.t0;
+      item_first += s.it.t1 - s.it.t0 + EXTRA;
       off = 0;
       if (++blk >= pa_blocks<ROWS>(p, s.r)) {
         blk = 0;
@@ -315,14 +317,14 @@ struct PaWalk {
 VVLI_DEV int pa_slot(const PaSeg& s) { return s.at_start ? 0 : 1; }
 
 // Called by one thread per CTA: what the combine kernel does for it.
+template <int EXTRA>
 VVLI_DEV void pa_describe(const PaParams& p, const PaShare& sh, const PaSeg* s) {
   PaDesc d{};
   if (s && !s->starts && s->ends) {
-    const long long wide = sh.more * (sh.each + 1);
-    const long long j = s->item_first < wide ? pa_div(s->item_first, sh.each + 1)
-                                             : sh.more + pa_div(s->item_first - wide, sh.each);
+    const long long tile = s->item_first + EXTRA, wide = sh.more * (sh.each + 1);  // the unit of the item's first tile
+    const long long j = tile < wide ? pa_div(tile, sh.each + 1) : sh.more + pa_div(tile - wide, sh.each);
     d.finish = 1, d.h = s->h, d.blk = s->blk, d.row0 = s->r.row0, d.rows = s->it.rows;
-    d.first = static_cast<int>(j), d.slot = pa_start(sh, j) == s->item_first ? 0 : 1;  // its second slot unless its share starts there
+    d.first = static_cast<int>(j), d.slot = pa_start(sh, j) >= s->item_first ? 0 : 1;  // its second slot unless its share starts there
   }
   p.desc[blockIdx.x] = d;
 }

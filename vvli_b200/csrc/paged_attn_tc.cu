@@ -39,6 +39,9 @@ constexpr int kTcKeys = 128;     // keys of a tile
 constexpr int kTcTile = 128;     // rows of a tile: M
 constexpr int kTcRows = 256;     // rows of an item
 constexpr int kTcThreads = 384;
+// An item's start and end count as this many tiles (4,096 new tokens at head_dim 64:
+// 172 us with none, 155 with 1, 134 with 2, 127 with 3; others alike from 2 on).
+constexpr int kTcExtra = 3;
 constexpr float kTcRise = 8.0f;  // a row maximum's rise (log2) that rescales its output
 
 template <int D>
@@ -203,6 +206,9 @@ VVLI_DEV void tca_cap(const PaParams& p, float* s) {
   }
 }
 
+// The bounded wait, out of line: the MMA warp's loop stays short.
+__device__ __noinline__ bool tca_wait_long(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
+
 // An item of at most 128 rows would leave one row tile idle and the other
 // waiting for its own MMAs: both tiles then hold the same rows and take the key
 // tiles in turn (twins), and tile 1's sums are added to tile 0's at the end.
@@ -263,10 +269,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  pa_schedule<kTcRows, kTcKeys, kTcThreads>(p, share, reinterpret_cast<PaScratch<kTcThreads>*>(sm + L::part));  // has barriers
+  pa_schedule<kTcRows, kTcKeys, kTcExtra, kTcThreads>(p, share, reinterpret_cast<PaScratch<kTcThreads>*>(sm + L::part));  // has barriers
   tc_fence_after();
   const uint32_t tmem = *holder;
-  PaWalk<kTcRows, kTcKeys> walk(*share);
+  PaWalk<kTcRows, kTcKeys, kTcExtra> walk(*share);
   PaSeg sg;
   bool dead = false;  // a wait gave up: the rest is skipped
 
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int per_tile = kTcKeys >> p.shift;
       bool any = false;
       while (!dead && walk.next(p, sg)) {
-        if (!any && lane == 0) pa_describe(p, *share, &sg);
+        if (!any && lane == 0) pa_describe<kTcExtra>(p, *share, &sg);
         any = true;
         const int pg0 = (sg.t0 * kTcKeys) >> p.shift;
         int chunk = 0;  // lane l holds page pg0 + 32 chunk + l, and the one 32 further
@@ -309,7 +315,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      if (!any && lane == 0) pa_describe(p, *share, nullptr);
+      if (!any && lane == 0) pa_describe<kTcExtra>(p, *share, nullptr);
       // no copy of this CTA is in flight when it ends
       for (int k = max(0, n - ST); k < n; ++k) mbar_wait(&full[k % ST], (k / ST) & 1, p.err);
     } else if (warp == 10) {  // ---- clears the values past the visible keys, and hands every V tile on
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t q_par0 = 0, q_par1 = 0, p_par0 = 0, p_par1 = 0;  // parities of the next waits on q_full, p_half / p_full
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity & 1)) && !dead)
-          dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
+          dead = !__all_sync(0xffffffffu, tca_wait_long(bar, parity & 1, p.err));
       };
       auto issue_s = [&](int t, uint32_t stage) {
         const uint64_t a = dq + ((t * L::q_tile) >> 4), b = dk + stage * (L::kv >> 4);
