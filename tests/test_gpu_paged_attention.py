@@ -131,6 +131,30 @@ def test_max_new_only_picks_the_kernel(torch, max_new):
     check(torch, make(torch, 2, lens, 8, 2, 128, 64, torch.bfloat16), 64, max_new=max_new)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", [(8, 2), (7, 1)])
+def test_few_rows_over_one_to_many_tiles(torch, d, hq, hk):
+    # items of at most 128 rows in the kernel for many: one key tile, two, odd and even counts, whole and split
+    lens = [(n, min(n, 1 + i % 9)) for i, n in enumerate([1, 64, 127, 128, 129, 200, 256, 257, 300, 384, 385, 640, 641, 1500])]
+    for window in (0, 130):
+        check(torch, make(torch, d + hq, lens, hq, hk, d, 64, torch.bfloat16), 64, max_new=1000, window=window)
+    check(torch, make(torch, d, [(6000, 5)], hq, hk, d, 32, torch.float16), 32, max_new=1000)
+
+
+@pytest.mark.parametrize("max_new", [1, 10**6])
+def test_nan_rows_stay_apart(torch, max_new):
+    # a NaN query gives NaN (whole item or split over CTAs) and leaves the rows beside it alone
+    q, k, v, table, cu, seq = make(torch, 11, [(3000, 3), (70, 2)], 4, 2, 64, 16, torch.bfloat16, poison=False)
+    q[1, 2], q[4, 0] = math.nan, math.inf
+    from vvli_b200.paged import PagedAttention
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    out, lse = PagedAttention(4, 2, 64, 16)(q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), max_new, lse=True)
+    bad = torch.zeros(5, 4, dtype=torch.bool)
+    bad[1, 2] = bad[4, 0] = True
+    assert torch.equal(torch.isnan(out.cpu()).all(-1), bad) and torch.equal(torch.isnan(out.cpu()).any(-1), bad)
+    assert torch.equal(torch.isnan(lse.cpu()), bad)
+
+
 @pytest.mark.parametrize("max_new", [1, 10**6])
 def test_empty_rows_bad_pages_and_rows_behind(torch, max_new):
     # seq_len 0 (an unserved request), fewer keys than rows, entries outside the cache, lengths past the table

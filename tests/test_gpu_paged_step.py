@@ -1,0 +1,107 @@
+"""The paged operators together: speculative decoding steps of a one-layer model, with page plans, rejected
+drafts and requests that come and go, against the dense computation in 64 bits.  Needs a B200."""
+
+import math
+
+import pytest
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HQ, HK, D, H, V, PAGE = 8, 2, 64, 128, 97, 16
+
+
+class Model:
+    """Embedding, one attention layer with q / k norms and rotation, and an LM head, in bf16 weights."""
+
+    def __init__(self, torch):
+        g = torch.Generator().manual_seed(7)
+        rnd = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[-1])).to(torch.bfloat16)  # noqa: E731
+        self.embed = torch.randn(V, H, generator=g).to(torch.bfloat16)
+        self.wqkv, self.wo, self.head = rnd((HQ + 2 * HK) * D, H), rnd(H, HQ * D), rnd(V, H) * 3
+        self.qn, self.kn = ((1 + 0.2 * torch.randn(D, generator=g)).to(torch.bfloat16) for _ in range(2))
+        self.freq = 10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))
+
+    def dense(self, torch, tokens):
+        """Attention rows and probabilities of every position of one token list, in 64 bits."""
+        x = self.embed[tokens].double()
+        qkv = x @ self.wqkv.double().T
+        n, pos = len(tokens), torch.arange(len(tokens))
+        q, k, v = (qkv[:, a * D:b * D].view(n, b - a, D) for a, b in ((0, HQ), (HQ, HQ + HK), (HQ + HK, HQ + 2 * HK)))
+        q = ref.qk_rows(q, self.qn, "head", 1e-6, pos, self.freq, False)
+        k = ref.qk_rows(k, self.kn, "head", 1e-6, pos, self.freq, False)
+        k, v = (y.repeat_interleave(HQ // HK, 1) for y in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q, k) / math.sqrt(D)
+        s = s.masked_fill(pos[None, None, :] > pos[None, :, None], -math.inf)
+        a = torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), v)
+        return a, torch.softmax((x + a.reshape(n, -1) @ self.wo.double().T) @ self.head.double().T, -1)
+
+
+def test_speculative_steps():
+    import torch
+    from vvli_b200.paged import PagedAttention, plan_step, qk_norm_rope_write
+    from vvli_b200.speculative import verify_drafts
+    m = Model(torch)
+    dev = {n: getattr(m, n).cuda() for n in ("embed", "wqkv", "wo", "head", "qn", "kn", "freq")}
+    g = torch.Generator().manual_seed(11)
+    B, pages, width, rows = 6, 40, 12, 256  # rows: the prompts (217 tokens) and 4 drafts each
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    caches = [torch.full((pages, HK, PAGE, D), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    free = ints(torch.randperm(pages, generator=g).tolist())
+    count, owned, table = ints([pages]), ints([0] * B), ints([[-1] * width] * B)
+    attention = PagedAttention(HQ, HK, D, PAGE)
+    history = [torch.randint(0, V, (n,), generator=g).tolist() for n in (1, 30, 64, 17, 5, 100)]  # prompts
+    cached = [0] * B
+    accepted_ever = rejected_ever = 0
+    for step in range(7):
+        if step == 4:  # request 2 ends: its pages go back on the stack, and another takes its place
+            n, c = int(owned[2]), int(count)
+            free[c:c + n] = table[2, :n]
+            count += n
+            owned[2], cached[2], history[2] = 0, 0, torch.randint(0, V, (40,), generator=g).tolist()
+        # every request feeds what is not cached yet (a prompt, or the token drawn last) and up to 4 drafts
+        fed = [h[c:] for h, c in zip(history, cached)]
+        drafts = [torch.randint(0, V, (int(torch.randint(0, 5, (1,), generator=g)),), generator=g).tolist() for _ in fed]
+        exact = [m.dense(torch, h + d) for h, d in zip(history, drafts)]
+        for b, d in enumerate(drafts):  # some drafts that the target likes
+            if d and step % 2:
+                d[0] = int(exact[b][1][len(history[b]) - 1].argmax())
+        exact = [m.dense(torch, h + d) for h, d in zip(history, drafts)]
+        new = [len(f) + len(d) for f, d in zip(fed, drafts)]
+        tokens = sum((f + d for f, d in zip(fed, drafts)), [])
+        T = len(tokens)
+        plan = plan_step(ints(cached), ints(new), owned, table, free, count, PAGE, rows, inplace=True)
+        assert plan.status.tolist() == [0] * B and int(plan.cu_new[-1]) == T
+        x = torch.zeros(rows, H, dtype=torch.bfloat16, device="cuda")
+        x[:T] = dev["embed"][torch.tensor(tokens, device="cuda")]
+        qkv = x @ dev["wqkv"].T
+        q, k, v = (qkv[:, a * D:b * D].view(rows, b - a, D) for a, b in ((0, HQ), (HQ, HQ + HK), (HQ + HK, HQ + 2 * HK)))
+        q = qk_norm_rope_write(q, k, v, *caches, plan.slots, plan.positions, dev["freq"], dev["qn"], dev["kn"])
+        out = attention(q, *caches, table, plan.cu_new, plan.seq_len, max(new))[:T]
+        probs = torch.softmax((x[:T].float() + out.reshape(T, -1).float() @ dev["wo"].float().T) @ dev["head"].float().T, -1)
+        # q, k, v are rounded to bf16 twice (projection, norm), the probabilities and the output once: each
+        # half a step (2^-8) of its value, which the softmax of scores of about 1 passes on about once
+        want = torch.cat([a[-n:] for (a, _), n in zip(exact, new)])
+        assert float((out.cpu().double() - want).norm() / want.norm()) < 6 * 2.0**-8
+        # verification of the drafts: row r of request b is judged from the last fed token on
+        starts = plan.cu_new.tolist()
+        judged = [r for b in range(B) for r in range(starts[b] + len(fed[b]) - 1, starts[b + 1])]
+        cu = [0]
+        for d in drafts:
+            cu.append(cu[-1] + len(d) + 1)
+        target = probs[torch.tensor(judged, device="cuda")].contiguous()
+        want_p = torch.cat([p[-(len(d) + 1):] for (_, p), d in zip(exact, drafts)])
+        assert float((target.cpu().double() - want_p).abs().max()) < 0.05
+        toks = ints([tokens[r] for r in judged])
+        ua, us = torch.rand(len(judged), generator=g), torch.rand(B, generator=g)
+        acc, emitted = verify_drafts(target, None, toks, ints(cu), ua.cuda(), us.cuda())
+        want_acc, want_out = ref.verify(target.cpu(), None, toks.cpu(), cu, ua, us)
+        assert acc.tolist() == want_acc and emitted.tolist() == want_out
+        for b in range(B):
+            n = want_acc[b]
+            cached[b] = len(history[b]) + n  # rejected drafts' slots and pages are simply used again
+            history[b] = history[b] + want_out[cu[b]:cu[b] + n + 1]
+            accepted_ever += n
+            rejected_ever += len(drafts[b]) - n
+    assert accepted_ever > 3 and rejected_ever > 3 and attention.status() == 0

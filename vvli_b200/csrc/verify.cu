@@ -28,6 +28,7 @@ namespace {
 constexpr int kVerThreads = 256;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerCluster = 8;
+constexpr int kVerRun = 12;  // values of a thread's run held in registers: the whole run up to 196,608 tokens
 constexpr int kVerUnroll = 4;  // loads in flight per lane and row
 
 VVLI_DEV uint32_t ver_cluster_rank() {
@@ -56,16 +57,44 @@ struct Weights {
     return w > 0.0 && i != skip ? w : 0.0;  // NaN: 0
   }
   VVLI_DEV double at(int i) const { return of(t[i], d ? d[i] : 0.f, i); }
-  // Four values from i on, zeros from `end` on (i a multiple of 4, rows 16-byte aligned).
-  VVLI_DEV float4 load4(const float* row, int i, int end) const {
-    if (!row || i >= end) return make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i + 4 <= end) return *reinterpret_cast<const float4*>(row + i);
-    return make_float4(row[i], i + 1 < end ? row[i + 1] : 0.f, i + 2 < end ? row[i + 2] : 0.f, 0.f);
-  }
-  VVLI_DEV double of4(const float4& a, const float4& b, int i) const {
-    return (of(a.x, b.x, i) + of(a.y, b.y, i + 1)) + (of(a.z, b.z, i + 2) + of(a.w, b.w, i + 3));
-  }
 };
+
+// This lane's share of the weights [s0, s1): whole batches of kVerUnroll loads
+// without a branch between them, so that all are in flight, then the rest.
+template <int VEC, bool DRAFT>
+VVLI_DEV double slice_sum(const Weights& w, int s0, int s1) {
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+  int i = s0 + VEC * lane;
+  if constexpr (VEC == 4) {
+    for (; i + 128 * (kVerUnroll - 1) + 4 <= s1; i += 128 * kVerUnroll) {
+      float4 x[kVerUnroll], y[kVerUnroll];
+#pragma unroll
+      for (int u = 0; u < kVerUnroll; ++u) {
+        x[u] = *reinterpret_cast<const float4*>(w.t + i + 128 * u);
+        y[u] = DRAFT ? *reinterpret_cast<const float4*>(w.d + i + 128 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < kVerUnroll; ++u) {
+        const int k = i + 128 * u;
+        sum += (w.of(x[u].x, y[u].x, k) + w.of(x[u].y, y[u].y, k + 1)) +
+               (w.of(x[u].z, y[u].z, k + 2) + w.of(x[u].w, y[u].w, k + 3));
+      }
+    }
+    for (; i < s1; i += 128)
+      for (int k = i; k < min(i + 4, s1); ++k) sum += w.of(w.t[k], DRAFT ? w.d[k] : 0.f, k);
+  } else {
+    for (; i + 32 * (kVerUnroll - 1) < s1; i += 32 * kVerUnroll) {
+      float x[kVerUnroll], y[kVerUnroll];
+#pragma unroll
+      for (int u = 0; u < kVerUnroll; ++u) x[u] = w.t[i + 32 * u], y[u] = DRAFT ? w.d[i + 32 * u] : 0.f;
+#pragma unroll
+      for (int u = 0; u < kVerUnroll; ++u) sum += w.of(x[u], y[u], i + 32 * u);
+    }
+    for (; i < s1; i += 32) sum += w.of(w.t[i], DRAFT ? w.d[i] : 0.f, i);
+  }
+  return sum;
+}
 
 VVLI_DEV double warp_sum_f64(double v) {
 #pragma unroll
@@ -75,7 +104,7 @@ VVLI_DEV double warp_sum_f64(double v) {
 
 // VEC: 4 when every row starts on a 16-byte boundary, else 1.
 template <int VEC>
-__global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_args p) {
+__global__ void __launch_bounds__(kVerThreads, 4) verify_kernel(const vvli_verify_args p) {
   __shared__ double warp_part[kVerWarps];
   __shared__ double scan_part[kVerWarps];
   __shared__ double cta_part[2];  // this CTA's slice sum, by attempt (read by the cluster)
@@ -131,27 +160,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
   int chosen = -1;  // CTA that holds the threshold
   double thr = 0.0;
   for (int attempt = 0; attempt < 2; ++attempt) {
-    double sum = 0.0;
-    if constexpr (VEC == 4) {
-      for (int i0 = s0 + 4 * lane; i0 < s1; i0 += 128 * kVerUnroll) {
-        float4 x[kVerUnroll], y[kVerUnroll];
-#pragma unroll
-        for (int u = 0; u < kVerUnroll; ++u) x[u] = w.load4(w.t, i0 + 128 * u, s1), y[u] = w.load4(w.d, i0 + 128 * u, s1);
-#pragma unroll
-        for (int u = 0; u < kVerUnroll; ++u) sum += w.of4(x[u], y[u], i0 + 128 * u);
-      }
-    } else {
-      for (int i0 = s0 + lane; i0 < s1; i0 += 32 * kVerUnroll) {
-        float x[kVerUnroll], y[kVerUnroll];
-#pragma unroll
-        for (int u = 0; u < kVerUnroll; ++u) {
-          const int i = i0 + 32 * u;
-          x[u] = i < s1 ? w.t[i] : 0.f, y[u] = w.d && i < s1 ? w.d[i] : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < kVerUnroll; ++u) sum += w.of(x[u], y[u], i0 + 32 * u);
-      }
-    }
+    const double sum = w.d ? slice_sum<VEC, true>(w, s0, s1) : slice_sum<VEC, false>(w, s0, s1);
     mine = warp_sum_f64(sum);
     if (lane == 0) warp_part[warp] = mine;
     __syncthreads();
@@ -201,15 +210,15 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
   const int per = (c1 - c0 + kVerThreads - 1) / kVerThreads;
   const int b0 = min(c0 + tid * per, c1), b1 = min(b0 + per, c1);
   double sum = 0.0;
-  for (int i0 = b0; i0 < b1; i0 += kVerUnroll) {
-    float x[kVerUnroll], y[kVerUnroll];
+  float x[kVerRun], y[kVerRun];  // the run, or its last values where it is longer
+  for (int i0 = b0; i0 < b1; i0 += kVerRun) {
 #pragma unroll
-    for (int u = 0; u < kVerUnroll; ++u) {
+    for (int u = 0; u < kVerRun; ++u) {
       const int i = i0 + u;
       x[u] = i < b1 ? w.t[i] : 0.f, y[u] = w.d && i < b1 ? w.d[i] : 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < kVerUnroll; ++u) sum += w.of(x[u], y[u], i0 + u);
+    for (int u = 0; u < kVerRun; ++u) sum += w.of(x[u], y[u], i0 + u);
   }
   double c = sum;
 #pragma unroll
@@ -239,12 +248,18 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const vvli_verify_a
   if (tid != owner) return;
   int best = c0;  // no weight at all: the slice's first index (0: the draw falls to the first slice)
   run = lead + c - sum;
-  for (int i = b0; i < b1; ++i) {
-    const double x = w.at(i);
-    if (x <= 0.0) continue;
-    best = i;
-    run += x;
-    if (run > thr) break;
+  bool over = false;
+  if (per <= kVerRun) {
+#pragma unroll
+    for (int u = 0; u < kVerRun; ++u) {
+      const double v = w.of(x[u], y[u], b0 + u);
+      if (v > 0.0 && !over) best = b0 + u, run += v, over = run > thr;
+    }
+  } else {
+    for (int i = b0; i < b1 && !over; ++i) {
+      const double v = w.at(i);
+      if (v > 0.0) best = i, run += v, over = run > thr;
+    }
   }
   p.out_tokens[row] = best;
 }
