@@ -581,8 +581,9 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  *   lse = ln(sum_j exp(s_j)).
  * q head g uses kv head g / (q_heads / kv_heads).  A row that sees no key
  * (p < 0) gets out 0 and lse -inf; rows from cu_new[requests] on are left as
- * they were.  What the cache holds past a request's seq_len is never used,
- * whatever its bits.  Keys whose table entry is outside [0, pages) count as
+ * they were.  What a row does not see does not reach it, whatever its bits
+ * (infinities and NaN among them), and what the cache holds past a request's
+ * seq_len is never used.  Keys whose table entry is outside [0, pages) count as
  * zero keys and values.  cu_new must not decrease and is cut at `tokens`,
  * seq_len at table_width * page_size.  Products of 16-bit values summed in fp32; the
  * probabilities enter the second product rounded to the 16-bit type, relative

@@ -131,6 +131,30 @@ def test_max_new_only_picks_the_kernel(torch, max_new):
     check(torch, make(torch, 2, lens, 8, 2, 128, 64, torch.bfloat16), 64, max_new=max_new)
 
 
+@pytest.mark.parametrize("d,dtype,page", [(64, "bfloat16", 16), (128, "float16", 64), (128, "bfloat16", 128)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("max_new", [1, 5, 10**6])
+def test_hidden_values_that_are_not_finite(torch, d, dtype, page, window, max_new):
+    # infinities and NaN among the values: only rows that see the key have them, in its columns alone
+    from vvli_b200.paged import PagedAttention
+    lens = [(90, 5), (300, 200), (64, 64), (700, 3), (2000, 40), (130, 1)]
+    q, k, v, table, cu, seq = make(torch, 21, lens, 8, 2, d, page, getattr(torch, dtype), poison=False)
+    g = torch.Generator().manual_seed(5)
+    for b, (e, n) in enumerate(lens):
+        for i, value in enumerate((math.nan, math.inf, -math.inf, math.inf)):
+            key = e - 1 - int(torch.randint(0, min(e, n + 110), (1,), generator=g))
+            v[table[b][key // page], i % 2, key % page, int(torch.randint(0, d, (1,), generator=g))] = value
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    att = PagedAttention(8, 2, d, page, dtype=q.dtype, window=window)
+    out = att(q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), max_new).cpu().double()
+    want, _ = ref.attention(q, k, v, table, cu, seq, d**-0.5, window)
+    odd = ~torch.isfinite(want)
+    assert int(odd.sum()) > 100 and torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out[odd & ~torch.isnan(want)], want[odd & ~torch.isnan(want)])
+    half = torch.finfo(q.dtype).eps / 2
+    assert float((out - want)[~odd].norm() / want[~odd].norm()) < 2 * half  # as in check()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq,hk", [(8, 2), (7, 1)])
 def test_few_rows_over_one_to_many_tiles(torch, d, hq, hk):

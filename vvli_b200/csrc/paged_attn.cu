@@ -43,7 +43,8 @@ struct ShLayout {
   static constexpr uint32_t ml = merge + 8 * 16 * o_ld * 4;  // [8][16][2]
   static constexpr uint32_t bars = ml + 8 * 16 * 2 * 4;
   static constexpr uint32_t share = bars + 2 * stages * 8;
-  static constexpr uint32_t part = share + 64;          // schedule scratch
+  static constexpr uint32_t odd = share + 64;           // ranges of tiles with values that are not finite, [2][2]
+  static constexpr uint32_t part = odd + 64;          // schedule scratch
   static constexpr uint32_t smem = part + sizeof(PaScratch<kShThreads>) + 1024;  // + alignment slack
 };
 static_assert(sizeof(PaShare) <= 64, "the share fits its space");
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::bars);
   uint64_t* empty = full + ST;
   PaShare* share = reinterpret_cast<PaShare*>(sm + L::share);
+  int* odd = reinterpret_cast<int*>(sm + L::odd);  // first and last tile, by the segment's parity
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   grid_launch_dependents();  // the combine kernel waits for this grid's completion before reading
@@ -98,6 +100,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], RG == 1 ? 4 : 8);  // the warps that read a stage
     }
+    odd[0] = odd[2] = INT_MAX, odd[1] = odd[3] = -1;
     fence_barrier_init();
   }
   pa_schedule<ROWS, kShKeys, kShExtra, kShThreads>(p, share, reinterpret_cast<PaScratch<kShThreads>*>(sm + L::part));
@@ -168,8 +171,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
   };
   const uint32_t krow = row_off(kkey), vrow = L::kv + row_off(vkey);
 
-  int it = 0;
-  while (walk.next(p, sg)) {
+  int it = 0, seg = 0;
+  for (; walk.next(p, sg); ++seg) {
     uint32_t qf[D / 16][4];
     int pos[2];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2] = {0.f, 0.f};
@@ -272,14 +275,27 @@ __global__ void __launch_bounds__(kShThreads, 1)
                     (key + 1 >= sg.it.lo && key + 1 < sg.it.hi ? 0xffff0000u : 0u);
         }
       }
+      const bool uneven = border && min_pos < sg.it.hi - 1;  // some row sees keys here that another does not
+      uint32_t bad = 0;
 #pragma unroll
       for (int jj = 0; jj < D / 16; ++jj) {
         uint32_t vf[4];
         const int c = 2 * jj + (lane >> 4);
         ldsm4_t(kv + vrow + (c >> 3) * slice + (((c & 7) ^ (vkey & 7)) << 4), vf);
         if (cut) vf[0] &= keep[0], vf[1] &= keep[1], vf[2] &= keep[0], vf[3] &= keep[1];
+        if (uneven) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t b = pa_not_finite<T>(vf[i]);
+            vf[i] &= ~b, bad |= b;
+          }
+        }
         mma16816<T>(o[2 * jj], pf, vf[0], vf[1]);
         mma16816<T>(o[2 * jj + 1], pf, vf[2], vf[3]);
+      }
+      if (__any_sync(0xffffffffu, bad != 0) && lane == 0) {
+        atomicMin(&odd[2 * (seg & 1)], t);
+        atomicMax(&odd[2 * (seg & 1) + 1], t);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
@@ -301,6 +317,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
       *reinterpret_cast<float2*>(at + 8 * L::o_ld) = make_float2(o[i][2], o[i][3]);
     }
     named_barrier(kShBarrier, kShConsumers);
+    const int odd0 = odd[2 * (seg & 1)], odd1 = odd[2 * (seg & 1) + 1];
+    if (tid == 0) odd[2 * (~seg & 1)] = INT_MAX, odd[2 * (~seg & 1) + 1] = -1;  // the next segment's
     constexpr int PER = ROWS * D / kShConsumers;  // dims of a row a thread adds up
     constexpr int PARTS = 8 / RG;
     const int r = tid / (D / PER), e0 = tid % (D / PER) * PER;
@@ -325,8 +343,9 @@ __global__ void __launch_bounds__(kShThreads, 1)
           acc[e + 2] = fmaf(f, v.z, acc[e + 2]), acc[e + 3] = fmaf(f, v.w, acc[e + 3]);
         }
       }
+      const int pr = sg.blk * ROWS + r, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
+      if (odd1 >= odd0) pa_add_not_finite<T, D, kShKeys, PER>(p, sg, sg.r.pos0 + tok, e0, odd0, odd1, acc);
       if (sg.starts && sg.ends) {
-        const int pr = sg.blk * ROWS + r, tok = pa_div_g(p, pr), head = sg.h * p.G + pr - tok * p.G;
         const float inv = Ls > 0.f ? 1.0f / Ls : 0.f;
         uint16_t* dst = p.out + (sg.r.row0 + tok) * p.out_stride + static_cast<long long>(head) * D + e0;
 #pragma unroll
@@ -523,6 +542,7 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.q_stride = static_cast<long long>(a.q_stride), p.out_stride = static_cast<long long>(a.out_stride);
   p.q = static_cast<const uint16_t*>(a.q), p.out = static_cast<uint16_t*>(a.out);
   p.lse = a.lse, p.alibi = a.alibi;
+  p.v = static_cast<const uint16_t*>(a.v_cache), p.page_stride = static_cast<long long>(a.page_stride);
   p.table = a.block_table, p.cu = a.cu_new, p.seq = a.seq_len;
   char* ws = static_cast<char*>(a.workspace);
   p.err = reinterpret_cast<int*>(ws);

@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "op_common.cuh"
@@ -50,6 +51,8 @@ struct PaParams {
   float cap_y, cap_in, cap_log2;             // softcap: scale / cap; that times 2 log2(e); cap * log2(e), 0 without
   long long q_stride, out_stride;
   const uint16_t* q;
+  const uint16_t* v;                         // the value cache, pages page_stride elements apart
+  long long page_stride;
   uint16_t* out;
   float* lse;
   const float* alibi;
@@ -372,6 +375,42 @@ VVLI_DEV int pa_page(const PaParams& p, int b, int pg) {
   int id = -1;
   if (pg < p.width) id = __ldg(p.table + static_cast<size_t>(b) * p.width + pg);
   return id >= 0 && id < p.pages ? id : p.pages;
+}
+
+// ---------------------------------------------------------------- values that are not finite
+// The second product multiplies a row's zeros with the values it does not see,
+// and 0 times an infinity or NaN is no 0.  Where the rows of an item see
+// different keys of a tile, such values are therefore taken out of the tile in
+// shared memory, the tiles that had any are kept as a range, and what a row does
+// see of them is added to its sums at the end, from the cache.
+template <class T>
+VVLI_DEV uint32_t pa_not_finite(uint32_t w) {  // 0xffff in each half that is an infinity or NaN
+  const uint32_t m = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
+  return __vcmpeq2(w & m, m);
+}
+template <class T>
+VVLI_DEV float pa_half(uint32_t w, int i) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return i ? bf16_hi(w) : bf16_lo(w);
+  const __half2 v = *reinterpret_cast<const __half2*>(&w);
+  return i ? __high2float(v) : __low2float(v);
+}
+// Adds what the row at position pos sees of them in key tiles [f0, f1] of request b, N dims from e0 on.
+template <class T, int D, int KT, int N>
+VVLI_DEV void pa_add_not_finite(const PaParams& p, const PaSeg& s, int pos, int e0, int f0, int f1, float* o) {
+  const int end = min(pos + 1, min((f1 + 1) * KT, s.it.hi));
+#pragma unroll 1
+  for (int key = max(f0 * KT, p.window ? pos + 1 - p.window : 0); key < end; ++key) {
+    const int page = pa_page(p, s.b, key >> p.shift);
+    if (page == p.pages) continue;
+    const uint16_t* v = p.v + page * p.page_stride +
+                        ((static_cast<long long>(s.h) << p.shift) + (key & ((1 << p.shift) - 1))) * D + e0;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(v + i), m = pa_not_finite<T>(w);
+      if (m & 0xffffu) o[i] += pa_half<T>(w, 0);
+      if (m >> 16) o[i + 1] += pa_half<T>(w, 1);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host

@@ -51,7 +51,8 @@ struct TcaLayout {
   static constexpr uint32_t stages = 131072 / kv;      // 4 at D 128, 8 at D 64; keys and values in turn
   static constexpr uint32_t ring = 2 * q_tile;
   static constexpr uint32_t bars = ring + stages * kv;
-  static constexpr uint32_t share = bars + 320;        // 3 stages + 11 barriers and the TMEM address
+  static constexpr uint32_t odd = bars + 320;          // [8][2] tiles with values that are not finite, by segment
+  static constexpr uint32_t share = odd + 64;         // 3 stages + 11 barriers and the TMEM address
   static constexpr uint32_t part = share + 64;
   static constexpr uint32_t smem = part + sizeof(PaScratch<kTcThreads>) + 1024;  // + alignment slack
   static constexpr uint32_t o_col = 256;               // S_0 at column 0, S_1 at 128, O_t at 256 + D t
@@ -320,7 +321,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int k = max(0, n - ST); k < n; ++k) mbar_wait(&full[k % ST], (k / ST) & 1, p.err);
     } else if (warp == 10) {  // ---- clears the values past the visible keys, and hands every V tile on
       int n = 0;
-      while (!dead && walk.next(p, sg)) {
+      // A segment's range is written before its V tiles are handed on and read
+      // after their MMAs; this warp is at most the ring's four tiles ahead.
+      for (int seg = 0; !dead && walk.next(p, sg); ++seg) {
+        int* odd = reinterpret_cast<int*>(sm + L::odd) + 2 * (seg & 7);
+        if (lane == 0) odd[0] = INT_MAX, odd[1] = -1;
+        const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows), last_pos = sg.it.hi - 1;
         for (int t = sg.t0; t < sg.t1; ++t, n += 2) {
           const int s = (n + 1) % ST;
           dead = !__all_sync(0xffffffffu, mbar_wait(&full[s], ((n + 1) / ST) & 1, p.err));
@@ -334,6 +340,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             tca_fence_async();
             __syncwarp();
+          }
+          // some row sees keys here that another does not
+          if (first_pos < last_pos && ((t + 1) * kTcKeys - 1 > first_pos || (p.window && t * kTcKeys <= last_pos - p.window))) {
+            uint4* v = reinterpret_cast<uint4*>(sm + L::ring + s * L::kv);
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int i = lane; i < kTcKeys * (D / 8); i += 32) {
+              uint4 w = v[i];
+              const uint4 b = make_uint4(pa_not_finite<T>(w.x), pa_not_finite<T>(w.y), pa_not_finite<T>(w.z), pa_not_finite<T>(w.w));
+              if (b.x | b.y | b.z | b.w) v[i] = make_uint4(w.x & ~b.x, w.y & ~b.y, w.z & ~b.z, w.w & ~b.w), any = 1;
+            }
+            if (__any_sync(0xffffffffu, any)) {
+              tca_fence_async();
+              if (lane == 0) odd[0] = min(odd[0], t), odd[1] = t;
+              __syncwarp();
+            }
           }
           if (lane == 0) mbar_arrive(&v_ready[s]);
         }
@@ -460,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
       tc_fence_after();
     };
-    while (walk.next(p, sg)) {  // after a wait gave up too: the tiles' barriers below need all threads
+    for (int seg = 0; walk.next(p, sg); ++seg) {  // after a wait gave up too: the tiles' barriers below need all threads
       const int nt = tca_tiles<D>(p, sg, t);
       const bool twins = tca_twins<D>(sg);
       const int row0 = twins ? 0 : t * kTcTile, R = row0 + lane_row;  // row of the item
@@ -601,6 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool whole = sg.starts && sg.ends, mine = !dead && !(twins && t == 1);
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
       const float inv = l == 0.f ? 0.f : 1.0f / l;  // no visible key: zeros
+      const int2 odd = *reinterpret_cast<const int2*>(sm + L::odd + 8 * (seg & 7));
       if (live && mine) {
         if (whole) {
           if (p.lse)
@@ -628,6 +651,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               o[i + 2] = o[i + 2] * fold + v.z * other, o[i + 3] = o[i + 3] * fold + v.w * other;
             }
           }
+          if (odd.y >= odd.x) pa_add_not_finite<T, D, kTcKeys, 32>(p, sg, pos, 32 * c, odd.x, odd.y, o);
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
