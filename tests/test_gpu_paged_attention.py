@@ -125,6 +125,13 @@ def test_softcap_and_alibi(torch, softcap, with_alibi, window, long):
         check(torch, make(torch, 5, lens, 8, 2, d, 64, dtype, spread=4.0), 64, softcap=softcap, alibi=alibi, window=window)
 
 
+@pytest.mark.parametrize("softcap,spread,scale", [(50.0, 0.5, 0.125), (3.0, 1.0, 0.125), (20.0, 4.0, -0.2), (1.0, 30.0, 0.2),
+                                                  (1e-3, 1.0, 0.125), (1e7, 1.0, 0.125), (2e-5, 1.0, 1e-6)])
+def test_softcap_from_far_below_to_far_above_the_scores(torch, softcap, spread, scale):
+    for lens in ([(200, 150)], [(200, 2)]):
+        check(torch, make(torch, 31, lens, 4, 2, 64, 64, torch.bfloat16, spread=spread), 64, softcap=softcap, scale=scale)
+
+
 @pytest.mark.parametrize("max_new", [0, 1, 4, 300, 10**6])
 def test_max_new_only_picks_the_kernel(torch, max_new):
     lens = [(300, 120), (64, 1), (200, 7), (33, 33)]

@@ -536,7 +536,6 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.scale_log2 = static_cast<float>((p.negate ? -a.scale : a.scale) * kLog2e);
   if (a.softcap > 0.f) {
     p.cap_y = a.scale / a.softcap;
-    p.cap_in = static_cast<float>(static_cast<double>(a.scale) / a.softcap * 2.0 * kLog2e);
     p.cap_log2 = static_cast<float>(a.softcap * kLog2e);
   }
   p.q_stride = static_cast<long long>(a.q_stride), p.out_stride = static_cast<long long>(a.out_stride);

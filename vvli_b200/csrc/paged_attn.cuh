@@ -48,7 +48,7 @@ struct PaParams {
   int window;                                // 0: none
   float scale_log2;                          // scale * log2(e); its magnitude without a feature, then
   int negate;                                // the sign goes into q
-  float cap_y, cap_in, cap_log2;             // softcap: scale / cap; that times 2 log2(e); cap * log2(e), 0 without
+  float cap_y, cap_log2;                     // softcap: scale / cap; cap * log2(e), 0 without
   long long q_stride, out_stride;
   const uint16_t* q;
   const uint16_t* v;                         // the value cache, pages page_stride elements apart
@@ -334,18 +334,22 @@ VVLI_DEV void pa_describe(const PaParams& p, const PaShare& sh, const PaSeg* s) 
 
 // ---------------------------------------------------------------- scores
 // In log2 units, so that exp is one ex2: x = s * scale * log2(e), or with a
-// softcap cap * log2(e) * tanh(s * scale / cap), tanh(y) = 1 - 2 / (1 + e^2y)
-// (absolute error below 2^-22, where tanh.approx has 2^-11: a capped score of
-// 50 would be off by 0.02).
+// softcap cap * log2(e) * tanh(y), y = s * scale / cap.  tanh.approx is off by
+// 2^-11 (a capped score of 50 by 0.02); here tanh(y) = 1 - 2 / (1 + e^2y), and for
+// |y| <= 0.4, where that would lose the leading digits, y times the degree-3
+// minimax fit of tanh(y) / y in y^2 (relative error 1e-7).
 VVLI_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 VVLI_DEV float pa_capped(float s, const PaParams& p) {
+  const float y = s * p.cap_y, u = y * y;
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * p.cap_in)));
-  return p.cap_log2 * fmaf(-2.0f, r, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(y * 2.885390081777927f)));  // 2 log2(e)
+  float q = fmaf(-0.04755360336859857f, u, 0.13270976752811006f);
+  q = fmaf(fmaf(q, u, -0.3333136245857671f), u, 0.9999999019009012f);
+  return p.cap_log2 * (fabsf(y) <= 0.4f ? q * y : fmaf(-2.0f, r, 1.0f));
 }
 
 template <class T>
