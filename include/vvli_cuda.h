@@ -488,7 +488,7 @@ enum vvli_dtype {
  *   1 the free pages ran out at it (the pages that earlier unserved requests
  *     lack count as taken, so the outcome does not depend on their sizes' order)
  *   2 it needs more than table_width pages
- *   3 its rows end past max_tokens
+ *   3 its rows end past max_tokens (when that is not 0)
  * Outputs: cu_new [requests + 1] (exclusive sums of new_tokens: request b's
  * rows are cu_new[b] .. cu_new[b + 1]); seq_len[b] = context + new, 0 for an
  * unserved request; owned_out[b] and free_count_out, the new state (each may
@@ -592,7 +592,7 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * it picks the kernel, not the result (up to a rounding).  A call queues two
  * kernels.  Two calls that may run at the same time need a workspace each.
  * Limits: head_dim 64 or 128; q_heads a multiple of kv_heads, q_heads <= 512;
- * tokens * q_heads < 2^31; requests in [1, 65536]; window < 2^31; strides (elements) multiples of 8 and at least a
+ * tokens * q_heads <= 2^31 - 1025; requests in [1, 65536]; window < 2^31; strides (elements) multiples of 8 and at least a
  * row; 16-bit pointers 16-byte aligned; workspace 256-byte aligned.  The first
  * int32 of the workspace is set to VVLI_ERR_TIMEOUT if a bounded wait gave up
  * (never cleared; zero it before the first call to read it). */

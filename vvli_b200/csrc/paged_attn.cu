@@ -480,7 +480,7 @@ std::string check_attn(const vvli_paged_attn_args* a) {
   if (a->head_dim != 64 && a->head_dim != 128) return "head_dim must be 64 or 128";
   if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads > 512 || a->q_heads % a->kv_heads)
     return "q_heads must be a multiple of kv_heads in [1, 512]";
-  if (a->tokens > INT_MAX / a->q_heads) return "tokens * q_heads must be below 2^31";
+  if (a->tokens > (INT_MAX - 1024) / a->q_heads) return "tokens * q_heads must be at most 2^31 - 1025";
   const std::string page = check_page_size(a->page_size);
   if (!page.empty()) return page;
   if (a->pages < 1 || a->pages > static_cast<uint64_t>(INT_MAX) / a->page_size)

@@ -20,7 +20,6 @@ None); tensors used on another stream than their own must outlive that work.
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
@@ -85,7 +84,7 @@ def _heads(who: str, name: str, x, shape, dtype, index: int) -> int:
         raise ValueError(f"{who}: {name} must be a {list(shape)} {dtype} tensor on cuda:{index}")
     apart, sh, sd = x.stride()
     n, h, d = shape
-    if (sd != 1 and d > 1) or (sh != d and h > 1):
+    if (sd != 1 or sh != d) and ((sd != 1 and d > 1) or (sh != d and h > 1)):
         raise ValueError(f"{who}: the rows of {name} must be contiguous")
     return apart if n > 1 else h * d
 
@@ -127,12 +126,12 @@ def plan_step(context, new, owned, block_table, free_pages, free_count, page_siz
     slots = pos + 4 * max_tokens
     own = slots + 4 * max_tokens
     own_in, free_in = _ints(who, "owned", owned, dev, B), _ints(who, "free_count", free_count, dev, 1)
-    a = _abi.CPagedPlanArgs(
+    a = _abi.pack_paged_plan(
         B, page_size, free_pages.numel(), block_table.shape[1], max_tokens, _ints(who, "context", context, dev),
         _ints(who, "new", new, dev, B), own_in, _ints(who, "block_table", block_table, dev),
         _ints(who, "free_pages", free_pages, dev), free_in, cu, seq, pos, slots, own_in if inplace else own,
         free_in if inplace else own + 4 * B, own + 4 * B + 4)
-    check(_abi.lib().vvli_cuda_paged_plan(dev, ctypes.byref(a), _stream(dev, stream)))
+    check(_abi.lib().vvli_cuda_paged_plan(dev, a, _stream(dev, stream)))
     out = buf.split_with_sizes(sizes)
     if inplace:
         out = (*out[:4], owned, free_count, out[6])
@@ -161,7 +160,7 @@ def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_fre
     ks = _heads(who, "k", k, (T, hk, d), dtype, dev)
     vs = _heads(who, "v", v, (T, hk, d), dtype, dev)
     pages, page_size, page_stride = _cache_layout(who, k_cache, v_cache, hk, d, dtype, dev)
-    pairs = freq = pos = qw = kw = None
+    pairs = freq = pos = qw = kw = 0  # addresses: 0 is null
     if inv_freq is not None:
         if inv_freq.dtype is not torch.float64 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
             raise ValueError(f"qk_norm_rope_write: inv_freq must be a contiguous float64 tensor on cuda:{dev}")
@@ -178,12 +177,12 @@ def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_fre
         out, os = _empty(shape, dtype, q.device, stream), hq * d
     else:
         os = _heads(who, "out", out, shape, dtype, dev)
-    a = _abi.CQkRopeArgs(
-        T, hq, hk, d, pairs or 0, page_size, pages, page_stride, qs, ks, vs, os, _DTYPES[dtype], _NORMS[norm],
+    a = _abi.pack_qk_rope(
+        T, hq, hk, d, pairs, page_size, pages, page_stride, qs, ks, vs, os, _DTYPES[dtype], _NORMS[norm],
         1 if interleaved else 0, eps, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
         v_cache.data_ptr(), qw, kw, pos, _ints(who, "slots", slots, dev, T), freq)
     if T:
-        check(_abi.lib().vvli_cuda_qk_rope_write(dev, ctypes.byref(a), _stream(dev, stream)))
+        check(_abi.lib().vvli_cuda_qk_rope_write(dev, a, _stream(dev, stream)))
     return out
 
 
@@ -228,7 +227,7 @@ class PagedAttention:
         self.softcap, self.window = float(softcap), int(window)
         if self.window < 0:
             raise ValueError("PagedAttention: window must be >= 0")
-        self._type, self._alibi = _DTYPES[dtype], None if alibi is None else alibi.data_ptr()
+        self._type, self._alibi = _DTYPES[dtype], 0 if alibi is None else alibi.data_ptr()
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._ws[:4].zero_()
         self._ws_at, self._ws_bytes = self._ws.data_ptr(), need
@@ -251,7 +250,7 @@ class PagedAttention:
             out, os = _empty_like(q, stream), hq * d
         else:
             os = _heads(who, "out", out, shape, dtype, dev)
-        lp = None
+        lp = 0
         if lse is True:
             lse = _empty((T, hq), torch.float32, self.device, stream)
             lp = lse.data_ptr()
@@ -259,12 +258,12 @@ class PagedAttention:
             if lse.dtype is not torch.float32 or lse.get_device() != dev or lse.shape != (T, hq) or not lse.is_contiguous():
                 raise ValueError(f"PagedAttention: lse must be a contiguous [{T}][{hq}] float32 tensor on cuda:{dev}")
             lp = lse.data_ptr()
-        a = _abi.CPagedAttnArgs(
+        a = _abi.pack_paged_attn(
             B, T, hq, self.kv_heads, d, page_size, pages, page_stride, block_table.shape[1], qs, os, max(0, max_new),
             self.window, self._type, self.scale, self.softcap, 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             out.data_ptr(), lp, self._alibi, _ints(who, "block_table", block_table, dev),
             _ints(who, "cu_new", cu_new, dev, B + 1), _ints(who, "seq_len", seq_len, dev), self._ws_at, self._ws_bytes)
-        check(_abi.lib().vvli_cuda_paged_attention(dev, ctypes.byref(a), _stream(dev, stream)))
+        check(_abi.lib().vvli_cuda_paged_attention(dev, a, _stream(dev, stream)))
         return out if lse is False else (out, lse)
 
     def status(self) -> int:

@@ -8,8 +8,6 @@ so that the emitted tokens are distributed as the target's.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _abi
@@ -56,7 +54,7 @@ def verify_drafts(target, draft, tokens, cu_rows, u_accept, u_sample, stream=Non
             buf.zero_()
     else:
         at = buf.data_ptr()
-        a = _abi.CVerifyArgs(B, T, V, ts, ds, target.data_ptr(), None if draft is None else draft.data_ptr(), tok, cu, ua, us,
+        a = _abi.pack_verify(B, T, V, ts, ds, target.data_ptr(), 0 if draft is None else draft.data_ptr(), tok, cu, ua, us,
                              at, at + 4 * B)
-        check(_abi.lib().vvli_cuda_verify_drafts(dev, ctypes.byref(a), _stream(dev, stream)))
+        check(_abi.lib().vvli_cuda_verify_drafts(dev, a, _stream(dev, stream)))
     return buf.split_with_sizes((B, T))
