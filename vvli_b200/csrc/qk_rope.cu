@@ -26,6 +26,12 @@ namespace {
 
 constexpr int kQkMaxThreads = 256;
 constexpr int kQkMaxTokens = 8;  // tokens of a CTA
+// Tokens in flight, and CTAs per SM: 16,384 tokens of 48 heads of 128 took 73.6 us so,
+// 75 with five ahead, 80 to 82 with two CTAs or four (registers), 84 loading one ahead
+// into registers.
+constexpr int kQkAhead = 3;
+constexpr int kQkPerSm = 3;
+constexpr int kQkStages = kQkAhead + 1;
 
 template <class T>
 struct Pair16;
@@ -61,6 +67,14 @@ VVLI_DEV uint4 pack8(const float* v) {
                     Pair16<T>::store(v[6], v[7]));
 }
 VVLI_DEV uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+VVLI_DEV void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+VVLI_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+VVLI_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
 VVLI_DEV void st16(void* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
 
 struct QkDev {
@@ -81,8 +95,10 @@ struct QkDev {
 // in a warp).  CTA (x, y): tokens x * per_cta .. and part y of the heads;
 // a thread keeps its head and chunks, hence its weights, for all tokens.
 template <class T, int NORM, int LANES, bool PAIRED>
-__global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p) {
+__global__ void __launch_bounds__(kQkMaxThreads, kQkPerSm) qk_rope_kernel(const QkDev p) {
   extern __shared__ __align__(16) float2 turn[];  // [tokens of the CTA][pairs] cosine, sine
+  uint4* ring = reinterpret_cast<uint4*>(turn + ((p.per_cta * p.pairs + 1) & ~1));  // [kQkStages][2][threads]
+  __shared__ unsigned slots[kQkMaxTokens];
   __shared__ float row_sum[2][kQkMaxTokens][kQkMaxThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int t0 = blockIdx.x * p.per_cta, nt = min(p.per_cta, p.tokens - t0);
@@ -101,12 +117,18 @@ __global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p
     const uint16_t* src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
     const long long step = kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride;
     src += t0 * step + g * p.d;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    unsigned slot = 0;
-    if (live) {
-      a = ld16(src + c0), b = ld16(src + c1);
-      if (kind) slot = static_cast<unsigned>(p.slots[t0]);
-    }
+    // A thread's own chunks of the next kQkAhead tokens are on their way to its
+    // own places of shared memory, so that they take no registers.
+    auto ahead = [&](int t) {
+      if (live && t < nt) {
+        uint4* at = ring + (t % kQkStages) * 2 * threads + tid;
+        cp_async16(at, src + t * step + c0);
+        cp_async16(at + threads, src + t * step + c1);
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int t = 0; t < kQkAhead; ++t) ahead(t);
     uint4 wa, wb;  // this thread's weights
     if constexpr (NORM != VVLI_NORM_NONE) {
       const uint16_t* wp = kind == 1 ? p.k_weight : p.q_weight;
@@ -118,6 +140,7 @@ __global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p
       }
     }
     if (part == static_cast<int>(blockIdx.y)) {
+      if (tid < nt) slots[tid] = static_cast<unsigned>(p.slots[t0 + tid]);
       for (int i = tid; i < nt * p.pairs; i += threads) {
         const int t = i / p.pairs, f = i - t * p.pairs;
         constexpr double kInvTwoPi = 0.15915494309189533576888;
@@ -154,13 +177,14 @@ __global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p
     uint16_t* const out = p.q_out + t0 * p.out_stride + g * p.d;
     uint16_t* const cache = kind == 1 ? p.k_cache : p.v_cache;
     for (int t = 0; t < nt; ++t) {
-      uint4 na = make_uint4(0, 0, 0, 0), nb = na;
-      unsigned nslot = 0;
-      src += step;
-      if (live && t + 1 < nt) {  // the next token's, before this one's work
-        na = ld16(src + c0), nb = ld16(src + c1);
-        if (kind) nslot = static_cast<unsigned>(p.slots[t0 + t + 1]);
+      cp_async_wait<kQkAhead - 1>();
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (live) {
+        const uint4* at = ring + (t % kQkStages) * 2 * threads + tid;
+        a = at[0], b = at[threads];
       }
+      ahead(t + kQkAhead);  // into the place of token t - 1
+      const unsigned slot = live && kind ? slots[t] : 0u;
       uint16_t* dst = nullptr;
       if (live && kind == 0)
         dst = out + t * p.out_stride;
@@ -203,7 +227,6 @@ __global__ void __launch_bounds__(kQkMaxThreads, 4) qk_rope_kernel(const QkDev p
         a = pack8<T>(x), b = pack8<T>(x + 8);
       }
       if (dst) st16(dst + c0, a), st16(dst + c1, b);
-      a = na, b = nb, slot = nslot;
     }
   }
 }
@@ -250,6 +273,7 @@ cudaError_t queue_lanes(const QkDev& p, size_t smem, cudaStream_t s) {
   const int heads = p.hq + 2 * p.hk, most = kQkMaxThreads / lanes;
   const int parts = (heads + most - 1) / most, each = (heads + parts - 1) / parts;
   const int threads = (each * lanes + 31) & ~31;
+  smem += static_cast<size_t>(kQkStages) * 2 * threads * sizeof(uint4);  // <= 8 + 32 KB
   const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, NORM == VVLI_NORM_ROW ? 1 : (heads + threads / lanes - 1) / (threads / lanes));
   switch (lanes) {
     case 1: qk_rope_kernel<T, NORM, 1, PAIRED><<<grid, threads, smem, s>>>(p); break;
@@ -290,7 +314,7 @@ cudaError_t queue_qk(const vvli_qk_rope_args& a, cudaStream_t s) {
   p.positions = a.positions, p.slots = a.slots, p.inv_freq = a.inv_freq;
   // Few tokens are spread over the SMs; many share a CTA's table and prologue.
   p.per_cta = p.tokens <= 256 ? 1 : p.tokens <= 1024 ? 2 : kQkMaxTokens;
-  const size_t smem = static_cast<size_t>(p.per_cta) * p.pairs * sizeof(float2);
+  const size_t smem = static_cast<size_t>((p.per_cta * p.pairs + 1) & ~1) * sizeof(float2);
   if (a.dtype == VVLI_BF16)
     return a.interleaved ? queue_norm<__nv_bfloat16, true>(p, a.norm, smem, s)
                          : queue_norm<__nv_bfloat16, false>(p, a.norm, smem, s);
