@@ -303,6 +303,27 @@ def test_repeats_bit_for_bit_captured_and_on_another_stream(torch, new):
     assert float((third.cpu().double() - want).norm() / want.norm()) < 2.0**-7
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("softcap,with_alibi", [(5.0, False), (50.0, True)])
+def test_softcap_repeats_bit_for_bit_between_other_calls(torch, d, softcap, with_alibi):
+    # what other calls left in shared memory past the last keys must not show, in the last bit either
+    from vvli_b200.paged import PagedAttention
+    r = random.Random(d)
+    lens = [(n + r.randint(0, 200), n) for n in (r.randint(1, 40) for _ in range(120))]
+    q, k, v, table, cu, seq = make(torch, 41, lens, 6, 3, d, 16, torch.bfloat16, poison=False)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    att = PagedAttention(6, 3, d, 16, softcap=softcap, alibi=torch.rand(6).cuda() if with_alibi else None)
+    args = (ints(table), ints(cu), ints(seq), 10**6)
+    mine, other = (q.cuda(), k.cuda(), v.cuda()), (8 * q.cuda(), 30 * k.cuda(), v.cuda())
+    first = att(*mine, *args, lse=True)
+    for i in range(12):
+        att(*other, *args)
+        if i % 3 == 0:
+            att(q.cuda(), torch.full_like(other[1], math.nan), other[2], *args)
+        again = att(*mine, *args, lse=True)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
 def test_wrapper_refusals(torch):
     from vvli_b200.errors import VvliError
     from vvli_b200.paged import PagedAttention

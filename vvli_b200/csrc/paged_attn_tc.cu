@@ -545,7 +545,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) tca_pin(s + 32 * c);
         const int key0 = (sg.t0 + (twins ? 2 * j + t : j)) * kTcKeys;
         const int lim = pos - key0;  // columns up to here are visible
-        if constexpr (FEAT & kPaCap) tca_cap(p, s);
+        const bool border = key0 + kTcKeys - 1 > first_pos || (p.window && key0 <= last_pos - p.window);  // uniform over the warp
+        const int low = p.window ? lim - p.window : -1;  // columns up to here are before the window
+        if constexpr (FEAT & kPaCap) {
+          if (border) {  // what is not visible (old shared memory past the last key) must not choose the formula
+#pragma unroll
+            for (int i = 0; i < 128; ++i) s[i] = i <= lim && i > low ? s[i] : 0.f;
+          }
+          tca_cap(p, s);
+        }
         if constexpr (FEAT & kPaAlibi) {
           const float2 sl = make_float2(slope, slope), at = make_float2(-static_cast<float>(lim), -static_cast<float>(lim));
           const float2 unit2 = make_float2(p.scale_log2, p.scale_log2);
@@ -558,8 +566,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             s[i] = x.x, s[i + 1] = x.y;
           }
         }
-        if (key0 + kTcKeys - 1 > first_pos || (p.window && key0 <= last_pos - p.window)) {  // uniform over the warp
-          const int low = p.window ? lim - p.window : -1;  // columns up to here are before the window
+        if (border) {
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] = i <= lim && i > low ? s[i] : -INFINITY;
         }
