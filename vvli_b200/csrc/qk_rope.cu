@@ -274,7 +274,7 @@ cudaError_t queue_lanes(const QkDev& p, size_t smem, cudaStream_t s) {
   const int parts = (heads + most - 1) / most, each = (heads + parts - 1) / parts;
   const int threads = (each * lanes + 31) & ~31;
   smem += static_cast<size_t>(kQkStages) * 2 * threads * sizeof(uint4);  // <= 8 + 32 KB
-  const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, NORM == VVLI_NORM_ROW ? 1 : (heads + threads / lanes - 1) / (threads / lanes));
+  const dim3 grid((static_cast<unsigned>(p.tokens) + p.per_cta - 1) / p.per_cta, NORM == VVLI_NORM_ROW ? 1 : (heads + threads / lanes - 1) / (threads / lanes));
   switch (lanes) {
     case 1: qk_rope_kernel<T, NORM, 1, PAIRED><<<grid, threads, smem, s>>>(p); break;
     case 2: qk_rope_kernel<T, NORM, 2, PAIRED><<<grid, threads, smem, s>>>(p); break;
