@@ -51,32 +51,32 @@ def _verify(name=None, requests=4, drafts=(1, 4), vocab=128256, one_hot=False, l
 def listed():
     return [
         # one chat sequence, one token a step: latency
-        _attention("attention one sequence", requests=1, ctx=(575, 575), lengths=1),
+        _attention("attention, one sequence", requests=1, ctx=(575, 575), lengths=1),
         # a full decode batch of long documents: the cache's bandwidth
-        _attention("attention long decode", requests=16, ctx=(24000, 32767), lengths=2),
+        _attention("attention, long decode", requests=16, ctx=(24000, 32767), lengths=2),
         # four drafted tokens and the last accepted one, odd group of seven heads
-        _attention("attention drafts", model="qwen2.5-0.5b", dtype="fp16", page=16, requests=48, ctx=(200, 4000),
+        _attention("attention, drafts", model="qwen2.5-0.5b", dtype="fp16", page=16, requests=48, ctx=(200, 4000),
                    new=(5, 5), lengths=3),
         # the second half of a long prompt
-        _attention("attention prompt chunk", requests=1, ctx=(4096, 4096), new=(4096, 4096), lengths=4),
+        _attention("attention, prompt chunk", requests=1, ctx=(4096, 4096), new=(4096, 4096), lengths=4),
         # chunks of prompts among decoding requests, capped scores and a sliding window
-        _attention("attention mixed window", model="llama3.2-1b", dtype="bf16", page=32, requests=16, ctx=(100, 5000),
+        _attention("attention, mixed window", model="llama3.2-1b", dtype="bf16", page=32, requests=16, ctx=(100, 5000),
                    new=(100, 700), chunk_every=4, window=1024, softcap=50.0, lengths=5),
         # one decode batch, norm over the whole row
-        _qk("qk decode batch", model="olmoe", tokens=16, norm="row"),
+        _qk("qk, decode batch", model="olmoe", tokens=16, norm="row"),
         # an odd prompt chunk, half of each head rotated in interleaved pairs, far positions
-        _qk("qk ragged chunk", model="qwen2.5-0.5b", dtype="fp16", page=16, tokens=777, interleaved=True, rotary=0.5,
+        _qk("qk, ragged chunk", model="qwen2.5-0.5b", dtype="fp16", page=16, tokens=777, interleaved=True, rotary=0.5,
             far=131072),
         # a long chunk
-        _qk("qk long chunk", tokens=16384, far=32768),
+        _qk("qk, long chunk", tokens=16384, far=32768),
         # a decode step of a small server
-        _plan("plan decode", requests=16, ctx=(0, 4096)),
+        _plan("plan, decode", requests=16, ctx=(0, 4096)),
         # a step of a big one: prompts arriving among decoding requests
-        _plan("plan arrivals", requests=1024, page=16, ctx=(0, 16384), new=(16, 1024), chunk_every=8, lengths=2),
+        _plan("plan, arrivals", requests=1024, page=16, ctx=(0, 16384), new=(16, 1024), chunk_every=8, lengths=2),
         # prompt-lookup drafts of a few sequences
-        _verify("verify lookup", requests=4, drafts=(0, 4), vocab=50304, one_hot=True),
+        _verify("verify, lookup", requests=4, drafts=(0, 4), vocab=50304, one_hot=True),
         # a batch with a draft model
-        _verify("verify batch", requests=64, drafts=(1, 5), vocab=151936, lengths=2),
+        _verify("verify, batch", requests=64, drafts=(1, 5), vocab=151936, lengths=2),
     ]
 
 
