@@ -586,8 +586,9 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * seq_len is never used.  Keys whose table entry is outside [0, pages) count as
  * zero keys and values.  cu_new must not decrease and is cut at `tokens`,
  * seq_len at table_width * page_size.  Products of 16-bit values summed in fp32; the
- * probabilities enter the second product rounded to the 16-bit type, relative
- * to the row's largest score; results do not depend on timing.
+ * probabilities enter the second product rounded to the 16-bit type (fp16: half a
+ * step of those down to 2^-25 of the row's largest, and none below 2^-36 of it);
+ * results do not depend on timing.
  * `max_new` is the longest request's new tokens as far as the caller knows:
  * it picks the kernel, not the result (up to a rounding).  A call queues two
  * kernels.  Two calls that may run at the same time need a workspace each.

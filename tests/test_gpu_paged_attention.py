@@ -348,3 +348,37 @@ def test_wrapper_refusals(torch):
     with pytest.raises(VvliError):
         PagedAttention(5, 2, 64, 16)(z(3, 5, 64), c, c, t, i[:3], i[:2], 1)
     assert att(q[:0], c, c, t, i[:3], i[:2], 1).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("gap", [12.0, 15.0, 18.0])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_dominant_keys_of_no_value_leave_the_others(torch, dtype, gap, new):
+    # keys `gap` above some 30,000 others, with values of zero: the output is what the others add up to.  Eight such
+    # keys (16 apart) in every 2,048, and as many requests as keep the SMs at work on whole ones, so that the
+    # others are summed beside one.
+    from vvli_b200.paged import PagedAttention
+    g = torch.Generator().manual_seed(17)
+    dtype = getattr(torch, dtype)
+    q, k, v, table, _, _ = make(torch, 17, [(30000, new)], 4, 2, 64, 64, dtype, poison=False)
+    q.fill_(2.0)  # a score is 16 times the key's one number
+    k.copy_(0.015 * (2 * torch.rand(k.shape[:3] + (1,), generator=g) - 1))
+    v.copy_(64 * (0.5 + torch.rand(v.shape, generator=g)))
+    for key in (first + 16 * i for first in range(0, 29900, 2048) for i in range(8)):
+        page = table[0][key // 64]
+        k[page, :, key % 64], v[page, :, key % 64] = gap / 16, 0.0
+    B = 80
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    out, lse = PagedAttention(4, 2, 64, 64, dtype=dtype)(
+        q.repeat(B, 1, 1).cuda(), k.cuda(), v.cuda(), ints(table * B), ints([new * b for b in range(B + 1)]),
+        ints([30000] * B), new, lse=True)
+    want, wlse = ref.attention(q, k, v, table, [0, new], [30000], 64**-0.5)
+    # Values of one sign, so the errors of the terms bound that of the sum, relative to it: the output's
+    # rounding, that of a probability (half a step; in fp16 e^-18.3 is 2^-26.4, held as 2^-15.4 at least, where
+    # a half's spacing is 2^-24: 2^-9.6), 2^-11 for score and exponential as in check(), and 2^-13 for fp32
+    # sums over 30,000 keys, 16 at a time.
+    half = torch.finfo(dtype).eps / 2
+    off = float(((out.cpu().double().view(B, new, 4, 64) - want).abs() / want).max())
+    assert off < half + max(half, 2.0**-9.6) + 2.0**-11 + 2.0**-13
+    off = float((lse.cpu().double().view(B, new, 4) - wlse).abs().max())
+    assert off < 2.0**-10

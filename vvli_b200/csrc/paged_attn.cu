@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(kShThreads, 1)
           o[i][2] *= alpha[1], o[i][3] *= alpha[1];
         }
       }
-      const float mu[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+      constexpr float kLift = pa_lift<T>(15.f);
+      const float mu[2] = {m[0] == -INFINITY ? 0.f : pa_reference(m[0], kLift),
+                           m[1] == -INFINITY ? 0.f : pa_reference(m[1], kLift)};
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       if (t4 == 0) {
-        mml[(warp * 16 + g + 8 * i) * 2] = m[i];
+        mml[(warp * 16 + g + 8 * i) * 2] = pa_reference(m[i], pa_lift<T>(15.f));
         mml[(warp * 16 + g + 8 * i) * 2 + 1] = l[i];
       }
     }

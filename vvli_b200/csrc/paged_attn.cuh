@@ -60,7 +60,7 @@ struct PaParams {
   // workspace
   int* err;
   PaDesc* desc;    // [kPaMaxCtas]
-  float* part_ml;  // [kPaMaxCtas][2][kPaMaxRows][2] running maximum (log2 units) and sum
+  float* part_ml;  // [kPaMaxCtas][2][kPaMaxRows][2] reference (the maximum, but see pa_lift; log2 units) and sum
   float* part_o;   // [kPaMaxCtas][2] sums of an item's rows: [rows][D], or [D / 4][rows][4] (256 rows, a thread each)
 };
 
@@ -351,6 +351,19 @@ VVLI_DEV float pa_capped(float s, const PaParams& p) {
   q = fmaf(fmaf(q, u, -0.3333136245857671f), u, 0.9999999019009012f);
   return p.cap_log2 * (fabsf(y) <= 0.4f ? q * y : fmaf(-2.0f, r, 1.0f));
 }
+
+// Probabilities are 2^(x - reference), and enter the second product in the 16-bit
+// type.  bf16 has fp32's exponents; fp16 loses bits below 2^-14 and holds nothing
+// below 2^-25, so there the reference is LIFT below the row's maximum: with it at
+// the maximum, 30,000 keys 18 (natural units) below a few dominant ones vanished from the
+// output while the sum counted them.  The sums and the log-sum-exp are relative
+// to the same reference.  LIFT bits and what a maximum may rise above its
+// reference stay below 2^16, fp16's end; from 2^22 on the difference would round.
+template <class T>
+constexpr float pa_lift(float fp16_bits) {
+  return std::is_same<T, __half>::value ? fp16_bits : 0.f;
+}
+VVLI_DEV float pa_reference(float m, float lift) { return fabsf(m) < 4194304.f ? m - lift : m; }
 
 template <class T>
 VVLI_DEV uint32_t pa_pack(float a, float b);

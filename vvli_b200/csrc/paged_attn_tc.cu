@@ -11,8 +11,8 @@
 //     row (a TMEM lane), so the online softmax needs no shuffles.  P, rounded
 //     to the 16-bit type, goes back over the same columns, from where it is the
 //     A operand of O_t += P_t V; O_t stays in TMEM.  A row's O is rescaled only
-//     when its maximum rises by more than 2^8 (P then stays below 2^8), which
-//     after a row's first tiles is rare.
+//     when its maximum rises by more than 2^8 (P then stays below 2^8; in fp16
+//     2^4 and 2^15), which after a row's first tiles is rare.
 //   * K and V tiles come by TMA, a box per page and 64-element slice, into a
 //     128 KB ring in the 128-byte-swizzled layout; V is read as it lies (keys by
 //     rows) through an MN-major descriptor, so nothing is transposed.
@@ -42,7 +42,9 @@ constexpr int kTcThreads = 384;
 // An item's start and end count as this many tiles (4,096 new tokens at head_dim 64:
 // 172 us with none, 155 with 1, 134 with 2, 127 with 3; others alike from 2 on).
 constexpr int kTcExtra = 3;
-constexpr float kTcRise = 8.0f;  // a row maximum's rise (log2) that rescales its output
+// A row maximum's rise (log2) that rescales its output: 2^8, in fp16 2^4 above a reference 2^11 below it (paged_attn.cuh).
+template <class T>
+constexpr float kTcRise = std::is_same<T, __half>::value ? 4.0f : 8.0f;
 
 template <int D>
 struct TcaLayout {
@@ -509,7 +511,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int pos = live ? sg.r.pos0 + tok : -1;
       const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows + row0);  // of this tile's first row
       const int last_pos = sg.it.hi - 1;
-      float m = -INFINITY, l = 0.f;
+      constexpr float kLift = pa_lift<T>(11.f);
+      float m = -INFINITY, l = 0.f;  // the row's reference, and its sum relative to it
       const float slope = (FEAT & kPaAlibi) && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
       if (nt > 0 && !dead) {
         // D / 8 lanes side by side read a row: 16-byte chunk c of rows i * (256 / D) + lane / (D / 8) of the warp's 32
@@ -579,10 +582,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
         const float unit = FEAT ? 1.0f : p.scale_log2;  // s * unit is in log2 units; > 0
         const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * unit;
-        const bool rise = mt > m + kTcRise;  // m = -inf: any finite mt
+        const bool rise = mt - m > kTcRise<T> + kLift;  // m = -inf: any finite mt; a difference, which is exact for large ones
         if (__any_sync(0xffffffffu, rise)) {
-          const float alpha = rise ? ex2(m - mt) : 1.0f;  // m = -inf: 0
-          if (rise) m = mt;
+          const float low_mt = pa_reference(mt, kLift);
+          const float alpha = rise ? ex2(m - low_mt) : 1.0f;  // m = -inf: 0
+          if (rise) m = low_mt;
           l *= alpha;
           if (j > 0) {
 #pragma unroll 1
