@@ -382,3 +382,30 @@ def test_dominant_keys_of_no_value_leave_the_others(torch, dtype, gap, new):
     assert off < half + max(half, 2.0**-9.6) + 2.0**-11 + 2.0**-13
     off = float((lse.cpu().double().view(B, new, 4) - wlse).abs().max())
     assert off < 2.0**-10
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 90])
+def test_values_that_are_not_finite_before_runs_of_narrow_items(torch, d, window):
+    # chunks of two row tiles with infinities and NaN among their values, each followed by many requests of one
+    # token (items that one row tile works on), so that every CTA has dozens of items, over 384 requests in all
+    from vvli_b200.paged import PagedAttention
+    r = random.Random(d)
+    lens = [(n + r.randint(0, 60), n) for n in (70 if i % 40 == 3 else 1 for i in range(1600))]
+    q, k, v, table, cu, seq = make(torch, 23, lens, 8, 2, d, 16, torch.bfloat16, poison=False)
+    for b, (e, n) in enumerate(lens):
+        for i, value in enumerate((math.nan, math.inf, -math.inf) if n > 1 else ()):
+            key = e - 1 - r.randrange(n)
+            v[table[b][key // 16], i % 2, key % 16, r.randrange(d)] = value
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    att = PagedAttention(8, 2, d, 16, window=window)
+    args = (q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), 10**6)
+    want, _ = ref.attention(q, k, v, table, cu, seq, d**-0.5, window)
+    odd = ~torch.isfinite(want)
+    assert int(odd.sum()) > 1000
+    for _ in range(3):
+        out = att(*args).cpu().double()
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out[odd & ~torch.isnan(want)], want[odd & ~torch.isnan(want)])
+        assert float((out - want)[~odd].norm() / want[~odd].norm()) < 2 * torch.finfo(q.dtype).eps / 2  # as in check()
+    assert att.status() == 0

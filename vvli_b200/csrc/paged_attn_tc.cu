@@ -39,6 +39,7 @@ constexpr int kTcKeys = 128;     // keys of a tile
 constexpr int kTcTile = 128;     // rows of a tile: M
 constexpr int kTcRows = 256;     // rows of an item
 constexpr int kTcThreads = 384;
+constexpr int kTcOdd = 8;        // segments of a row tile whose key tiles with values that are not finite are kept
 // An item's start and end count as this many tiles (4,096 new tokens at head_dim 64:
 // 172 us with none, 155 with 1, 134 with 2, 127 with 3; others alike from 2 on).
 constexpr int kTcExtra = 3;
@@ -53,12 +54,14 @@ struct TcaLayout {
   static constexpr uint32_t stages = 131072 / kv;      // 4 at D 128, 8 at D 64; keys and values in turn
   static constexpr uint32_t ring = 2 * q_tile;
   static constexpr uint32_t bars = ring + stages * kv;
-  static constexpr uint32_t odd = bars + 320;          // [8][2] tiles with values that are not finite, by segment
-  static constexpr uint32_t share = odd + 64;         // 3 stages + 11 barriers and the TMEM address
+  static constexpr uint32_t odd = bars + 320;            // after 3 stages + 11 barriers and the TMEM address
+  static constexpr uint32_t share = odd + 16 * kTcOdd;   // [2][kTcOdd] first and last tile with values that are not finite
   static constexpr uint32_t part = share + 64;
   static constexpr uint32_t smem = part + sizeof(PaScratch<kTcThreads>) + 1024;  // + alignment slack
   static constexpr uint32_t o_col = 256;               // S_0 at column 0, S_1 at 128, O_t at 256 + D t
   static constexpr uint32_t slice = 128 * 128;         // bytes of a 64-element slice of a 128-row tile
+  static_assert((3 * stages + 11) * 8 + 4 <= odd - bars, "the barriers and the TMEM address fit");
+  static_assert(stages / 2 + 2 <= kTcOdd, "no range is overwritten before it is read");
 };
 
 // K-major operands have both descriptors' defaults (tc_ptx.cuh); this one is
@@ -342,10 +345,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp == 10) {  // ---- clears the values past the visible keys, and hands every V tile on
       int n = 0;
       // A segment's range is written before its V tiles are handed on and read
-      // after their MMAs; this warp is at most the ring's four tiles ahead.
-      for (int seg = 0; !dead && walk.next(p, sg); ++seg) {
-        int* odd = reinterpret_cast<int*>(sm + L::odd) + 2 * (seg & 7);
-        if (lane == 0) odd[0] = INT_MAX, odd[1] = -1;
+      // after their MMAs, by each row tile that works on it; a row tile counts the
+      // segments that it works on, and has kTcOdd places for them.  When this warp
+      // comes to a row tile's segment W, the MMAs are done with all but the last
+      // stages / 2 tiles before it, so with its segment W - 1 - stages / 2, whose
+      // queries the row tile hands over after reading the range of the one before.
+      int worked[2] = {0, 0};
+      while (!dead && walk.next(p, sg)) {
+        int* odd[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          odd[t] = tca_tiles<D>(p, sg, t) > 0 ? reinterpret_cast<int*>(sm + L::odd) + 2 * (t * kTcOdd + worked[t]++ % kTcOdd) : nullptr;
+          if (odd[t] && lane == 0) odd[t][0] = INT_MAX, odd[t][1] = -1;
+        }
         const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows), last_pos = sg.it.hi - 1;
         for (int t = sg.t0; t < sg.t1; ++t, n += 2) {
           const int s = (n + 1) % ST;
@@ -373,7 +385,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (__any_sync(0xffffffffu, any)) {
               tca_fence_async();
-              if (lane == 0) odd[0] = min(odd[0], t), odd[1] = t;
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (odd[i] && lane == 0) odd[i][0] = min(odd[i][0], t), odd[i][1] = t;
               __syncwarp();
             }
           }
@@ -502,7 +516,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, p.err));
       tc_fence_after();
     };
-    for (int seg = 0; walk.next(p, sg); ++seg) {  // after a wait gave up too: the tiles' barriers below need all threads
+    int worked = 0;           // segments that this tile has worked on
+    while (walk.next(p, sg)) {  // after a wait gave up too: the tiles' barriers below need all threads
       const int nt = tca_tiles<D>(p, sg, t);
       const bool twins = tca_twins<D>(sg);
       const int row0 = twins ? 0 : t * kTcTile, R = row0 + lane_row;  // row of the item
@@ -652,7 +667,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool whole = sg.starts && sg.ends, mine = !dead && !(twins && t == 1);
       const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + pa_slot(sg);
       const float inv = l == 0.f ? 0.f : 1.0f / l;  // no visible key: zeros
-      const int2 odd = *reinterpret_cast<const int2*>(sm + L::odd + 8 * (seg & 7));
+      const int2 odd = *reinterpret_cast<const int2*>(sm + L::odd + 8 * (t * kTcOdd + worked % kTcOdd));
+      worked += nt > 0;
       if (live && mine) {
         if (whole) {
           if (p.lse)
