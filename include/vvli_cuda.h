@@ -636,7 +636,11 @@ int vvli_cuda_paged_attention(int device, const vvli_paged_attn_args* args, void
  * probabilities, with the random numbers given.  Request b has rows
  * r0 = cu_rows[b] .. r1 = cu_rows[b + 1]; row r holds the token that was fed
  * (tokens[r]) and the target's probabilities of the next one, so rows
- * r0 + 1 .. r1 - 1 carry the drafts.  Draft i (tokens[r0 + i + 1]) is accepted
+ * r0 + 1 .. r1 - 1 carry the drafts.  Every row after a request's first counts
+ * as a draft: cu_new of a step serves as cu_rows only where each request was
+ * planned and fed one known token and its drafts.  Of a prompt chunk only the
+ * rows from its last token on belong here, of a request with status != 0 none.
+ * Draft i (tokens[r0 + i + 1]) is accepted
  * while u_accept[r0 + i] * q < p, p = target[r0 + i][draft] and q =
  * draft[r0 + i][draft] (1 without draft probabilities: a drafter that does not
  * sample).  At the first rejection, row r, the token is drawn from

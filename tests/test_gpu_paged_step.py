@@ -105,3 +105,65 @@ def test_speculative_steps():
             accepted_ever += n
             rejected_ever += len(drafts[b]) - n
     assert accepted_ever > 3 and rejected_ever > 3 and attention.status() == 0
+
+
+def test_rows_to_judge_of_a_mixed_step():
+    # A decode token with drafts, a prompt's end with and without drafts, the middle of a prompt, a request that feeds
+    # nothing, and one that gets no pages: only rows from the last known token on are judged, of those that want a token.
+    import torch
+    from vvli_b200.paged import PagedAttention, plan_step, qk_norm_rope_write
+    from vvli_b200.speculative import verify_drafts
+    m = Model(torch)
+    dev = {n: getattr(m, n).cuda() for n in ("embed", "wqkv", "wo", "head", "qn", "kn", "freq")}
+    g = torch.Generator().manual_seed(21)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    history = [torch.randint(0, V, (n,), generator=g).tolist() for n in (20, 33, 50, 40, 5, 90)]
+    known, drafts = [1, 33, 30, 25, 0, 90], [3, 0, 2, 0, 0, 1]  # fed tokens before the drafts, and drafts
+    want_token = [True, True, True, False, False, True]       # request 3 has more of its prompt to come
+    B, rows, pages, width = len(history), 256, 13, 8          # the first five take 2 + 3 + 4 + 3 + 1 pages: none is left
+    cached = [len(h) - k for h, k in zip(history, known)]
+    fed = [h[len(h) - k:] + torch.randint(0, V, (n,), generator=g).tolist() for h, k, n in zip(history, known, drafts)]
+    table = torch.full((B, width), -1, dtype=torch.int32)
+    owned, order = [-(-c // PAGE) for c in cached], torch.randperm(pages, generator=g).to(torch.int32)
+    for b in range(B):
+        table[b, :owned[b]] = order[sum(owned[:b]):sum(owned[:b + 1])]
+    free = order[sum(owned):].cuda()
+    caches = [torch.zeros(pages, HK, PAGE, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for b in range(B):  # what is cached already
+        if cached[b]:
+            x = m.embed[torch.tensor(history[b][:cached[b]])].cuda()
+            k, v = ((x @ dev["wqkv"][a * D:(a + HK) * D].T).view(-1, HK, D) for a in (HQ, HQ + HK))
+            at = torch.arange(cached[b])
+            slots = (table[b][at // PAGE] * PAGE + at % PAGE).int().cuda()
+            q = torch.zeros(cached[b], HQ, D, dtype=torch.bfloat16, device="cuda")
+            qk_norm_rope_write(q, k, v, *caches, slots, at.int().cuda(), dev["freq"], dev["qn"], dev["kn"])
+    table = table.cuda()
+    new = [len(f) for f in fed]
+    step = plan_step(ints(cached), ints(new), ints(owned), table, free, ints([free.numel()]), PAGE, rows)
+    assert step.status.tolist() == [0, 0, 0, 0, 0, 1]
+    fed_tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    fed_tokens[:sum(new)] = ints(sum(fed, []))
+    x = dev["embed"][fed_tokens.long()]
+    qkv = x @ dev["wqkv"].T
+    q, k, v = (qkv[:, a * D:b * D].view(rows, b - a, D) for a, b in ((0, HQ), (HQ, HQ + HK), (HQ + HK, HQ + 2 * HK)))
+    q = qk_norm_rope_write(q, k, v, *caches, step.slots, step.positions, dev["freq"], dev["qn"], dev["kn"])
+    out = PagedAttention(HQ, HK, D, PAGE)(q, *caches, table, step.cu_new, step.seq_len, max(new))
+    requests, most = B, sum(n + 1 for n in drafts)
+    wanted = ints([n + 1 if w else 0 for n, w in zip(drafts, want_token)])
+    wanted = torch.where(step.status == 0, wanted, 0)
+    cu_rows = torch.nn.functional.pad(wanted.cumsum(0), (1, 0)).int()
+    i = torch.arange(most, device=wanted.device)
+    b = torch.searchsorted(cu_rows[1:], i, right=True).clamp(max=requests - 1)
+    judged = (step.cu_new[b + 1] - cu_rows[b + 1] + i).clamp(0, rows - 1)
+    ends = [sum(new[:b + 1]) for b in range(B)]
+    want_rows = sum((list(range(ends[b] - drafts[b] - 1, ends[b])) for b in (0, 1, 2)), [])
+    assert cu_rows.tolist() == [0, 4, 5, 8, 8, 8, 8] and judged[:8].tolist() == want_rows
+    target = torch.softmax((x[judged].float() + out[judged].reshape(most, -1).float() @ dev["wo"].float().T)
+                           @ dev["head"].float().T, -1)
+    exact = [m.dense(torch, h[:c] + f)[1][-(n + 1):] for h, c, f, n in zip(history, cached, fed, drafts)]
+    assert float((target[:8].cpu().double() - torch.cat(exact[:3])).abs().max()) < 0.05  # as above
+    ua, us = torch.rand(most, generator=g) * 0.1, torch.rand(B, generator=g)
+    accepted, tokens = verify_drafts(target, None, fed_tokens[judged], cu_rows, ua.cuda(), us.cuda())
+    want = ref.verify(target.cpu(), None, fed_tokens[judged].cpu(), cu_rows.tolist(), ua, us)
+    assert accepted.tolist() == want[0] and accepted.tolist()[3:] == [0, 0, 0] and tokens[:8].tolist() == want[1][:8]
+    assert all(tokens[a + n].item() >= 0 for a, n in zip((0, 4, 5), want[0]))  # a token for each that wants one

@@ -34,7 +34,10 @@ def verify_drafts(target, draft, tokens, cu_rows, u_accept, u_sample, stream=Non
     target [rows][vocab]: float32 probabilities after each fed token; draft:
     the drafter's, row r for the draft fed at row r + 1, or None for a drafter
     that does not sample; tokens [rows] int32: the fed tokens (request b's rows
-    are cu_rows[b] .. cu_rows[b + 1], the first one not a draft); u_accept
+    are cu_rows[b] .. cu_rows[b + 1], the first one not a draft, all others
+    drafts: of a prompt only the rows from its last token on, of a request that
+    plan_step did not serve none; a step's cu_new is such a cu_rows only where
+    every request was served and fed one known token and drafts); u_accept
     [rows] and u_sample [requests]: float32 uniform numbers in [0, 1).
     Returns (accepted [requests], out [rows]) int32: out holds the accepted
     drafts from cu_rows[b] on, then the drawn token, then -1; rows of no
