@@ -167,3 +167,55 @@ def test_rows_to_judge_of_a_mixed_step():
     want = ref.verify(target.cpu(), None, fed_tokens[judged].cpu(), cu_rows.tolist(), ua, us)
     assert accepted.tolist() == want[0] and accepted.tolist()[3:] == [0, 0, 0] and tokens[:8].tolist() == want[1][:8]
     assert all(tokens[a + n].item() >= 0 for a, n in zip((0, 4, 5), want[0]))  # a token for each that wants one
+
+
+# A fresh process: which kernels have run before is the point.
+CAPTURE = """
+import torch
+from vvli_b200.paged import PagedAttention, qk_norm_rope_write
+from vvli_b200.speculative import verify_drafts
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+g = torch.Generator(device="cuda").manual_seed(1)
+
+def call(dtype, d, n, softcap, norm, odd):
+    att = PagedAttention(4, 2, d, 16, dtype=dtype, softcap=softcap)
+    q, k, v = rnd(n, 4, d).to(dtype), rnd(n, 2, d).to(dtype), rnd(n, 2, d).to(dtype)
+    caches = [torch.zeros(20, 2, 16, d, dtype=dtype, device="cuda") for _ in range(2)]
+    at = torch.arange(n, device="cuda", dtype=torch.int32)
+    freq = 0.5 ** torch.arange(8, dtype=torch.float64, device="cuda")
+    table, cu, seq = ints([list(range(20))]), ints([0, n]), ints([n])
+    target = torch.softmax(rnd(3, 1000 + odd), -1)
+    tokens, cu3, ua, us = ints([1, 2, 3]), ints([0, 3]), torch.full((3,), 0.01, device="cuda"), torch.full((1,), 0.5, device="cuda")
+    def step():
+        x = qk_norm_rope_write(q, k, v, *caches, at, at, freq, norm=norm, interleaved=bool(odd))
+        return x, att(x, *caches, table, cu, seq, n), *verify_drafts(target, None, tokens, cu3, ua, us)
+    return step
+
+call(torch.bfloat16, 64, 1, 0.0, "none", 0)()
+torch.cuda.synchronize()
+for dtype, d, n, softcap, norm, odd in ((torch.bfloat16, 64, 200, 0.0, "head", 0), (torch.float16, 128, 300, 30.0, "row", 1),
+                                        (torch.float16, 64, 5, 0.0, "head", 1)):
+    step = call(dtype, d, n, softcap, norm, odd)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [x.clone() for x in got]
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+    assert float(got[1].float().abs().max()) > 0.1
+print("captured")
+"""
+
+
+def test_captures_of_variants_that_have_not_run():
+    # one call of each operator, then captures with other types, sizes, features and alignments
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and p.stdout.endswith("captured\n"), p.stderr[-2000:]

@@ -4,7 +4,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <exception>
+#include <mutex>
 #include <string>
 
 #include "../../include/vvli_cuda.h"
@@ -61,5 +63,23 @@ inline std::string check_page_size(uint64_t p) {
 }
 
 constexpr int kOpMaxDevices = 64;
+
+// What an operator does once per device.  Only success is kept: a setup that
+// failed (out of memory, say) is tried again by the next call.
+class SetupOnce {
+  std::atomic<bool> done_{false};
+  std::mutex mutex_;
+
+ public:
+  template <class Setup>
+  cudaError_t operator()(Setup setup) {
+    if (done_.load(std::memory_order_acquire)) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (done_.load(std::memory_order_relaxed)) return cudaSuccess;
+    const cudaError_t e = setup();
+    if (e == cudaSuccess) done_.store(true, std::memory_order_release);
+    return e;
+  }
+};
 
 }  // namespace vvli

@@ -442,20 +442,11 @@ __global__ void __launch_bounds__(256, ROWS == kPaMaxRows ? 4 : 2) paged_combine
         s.L == 0.f ? -INFINITY : (s.M + log2f(s.L)) * 0.69314718055994530942f;
 }
 
-template <class K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-}
-
 template <class T, int D, int RG, bool FEAT>
-cudaError_t launch_short(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
-  static std::once_flag once[kOpMaxDevices];
-  static cudaError_t ready[kOpMaxDevices];
-  std::call_once(once[device], [&] { ready[device] = allow_smem(paged_short_kernel<T, D, RG, FEAT>, ShLayout<D>::smem); });
-  cudaError_t e = ready[device];
+cudaError_t launch_short(const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
   const uint32_t rows = static_cast<uint32_t>(std::min<uint64_t>(a.page_size, kShKeys));
-  if (e == cudaSuccess) e = pa_tensor_map(&km, a.k_cache, a, rows, D / 64);
+  cudaError_t e = pa_tensor_map(&km, a.k_cache, a, rows, D / 64);
   if (e == cudaSuccess) e = pa_tensor_map(&vm, a.v_cache, a, rows, D / 64);
   if (e != cudaSuccess) return e;
   paged_short_kernel<T, D, RG, FEAT><<<ctas, kShThreads, ShLayout<D>::smem, s>>>(p, km, vm);
@@ -467,13 +458,49 @@ cudaError_t launch_short(int device, const PaParams& p, const vvli_paged_attn_ar
 // 32 would stream the request's keys again, and the tensor-core kernel's blocks
 // have 256 rows.
 template <class T, int D>
-cudaError_t queue_variant(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
+cudaError_t queue_variant(const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
   const bool feat = pa_features(p) != 0;
   if (a.max_new <= 16u / p.G)
-    return feat ? launch_short<T, D, 1, true>(device, p, a, ctas, s) : launch_short<T, D, 1, false>(device, p, a, ctas, s);
+    return feat ? launch_short<T, D, 1, true>(p, a, ctas, s) : launch_short<T, D, 1, false>(p, a, ctas, s);
   if (a.max_new <= 32u / p.G)
-    return feat ? launch_short<T, D, 2, true>(device, p, a, ctas, s) : launch_short<T, D, 2, false>(device, p, a, ctas, s);
-  return pa_queue_tc<T, D>(device, p, a, ctas, s);
+    return feat ? launch_short<T, D, 2, true>(p, a, ctas, s) : launch_short<T, D, 2, false>(p, a, ctas, s);
+  return pa_queue_tc<T, D>(p, a, ctas, s);
+}
+
+// Every kernel of a type and head_dim, loaded and allowed its shared memory.
+template <class T, int D>
+cudaError_t set_up_variants() {
+  cudaError_t e = allow_smem(paged_short_kernel<T, D, 1, false>, ShLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_short_kernel<T, D, 1, true>, ShLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_short_kernel<T, D, 2, false>, ShLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_short_kernel<T, D, 2, true>, ShLayout<D>::smem);
+  if (e == cudaSuccess) e = pa_set_up_tc<T, D>();
+  cudaFuncAttributes loaded;
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&loaded, paged_combine_kernel<T, D, 16>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&loaded, paged_combine_kernel<T, D, 32>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&loaded, paged_combine_kernel<T, D, kPaMaxRows>);
+  return e;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode = nullptr;  // set by the first setup
+
+// Once per device, for all types and head_dims: a call that is captured into a
+// graph then does no more than launch.
+cudaError_t set_up_device(int device, int* sms) {
+  cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+  cudaDriverEntryPointQueryResult found;
+  void* f = nullptr;
+  if (e == cudaSuccess) e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found);
+  if (e == cudaSuccess && found != cudaDriverEntryPointSuccess) e = cudaErrorNotSupported;
+  if (e == cudaSuccess) e = set_up_variants<__nv_bfloat16, 64>();
+  if (e == cudaSuccess) e = set_up_variants<__nv_bfloat16, 128>();
+  if (e == cudaSuccess) e = set_up_variants<__half, 64>();
+  if (e == cudaSuccess) e = set_up_variants<__half, 128>();
+  if (e == cudaSuccess) {
+    static std::once_flag once;  // devices are set up side by side
+    std::call_once(once, [&] { tensor_map_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f); });
+  }
+  return e;
 }
 
 std::string check_attn(const vvli_paged_attn_args* a) {
@@ -515,13 +542,11 @@ std::string check_attn(const vvli_paged_attn_args* a) {
 cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s) {
   if (a.tokens == 0) return cudaSuccess;
   if (device < 0 || device >= kOpMaxDevices) return cudaErrorInvalidDevice;
-  static std::once_flag once[kOpMaxDevices];
+  static SetupOnce setup[kOpMaxDevices];
   static int sms[kOpMaxDevices];
-  std::call_once(once[device], [&] {
-    if (cudaDeviceGetAttribute(&sms[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) sms[device] = 0;
-  });
+  const cudaError_t e = setup[device]([&] { return set_up_device(device, &sms[device]); });
+  if (e != cudaSuccess) return e;
   const int ctas = std::min(sms[device], kPaMaxCtas);
-  if (ctas <= 0) return cudaErrorInvalidDevice;
   PaParams p{};
   p.B = static_cast<int>(a.requests), p.T = static_cast<int>(a.tokens);
   p.hq = static_cast<int>(a.q_heads), p.hk = static_cast<int>(a.kv_heads), p.G = p.hq / p.hk;
@@ -552,10 +577,9 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.part_o = p.part_ml + static_cast<size_t>(kPaMaxCtas) * 2 * kPaMaxRows * 2;
   static_assert((256 + kPaMaxCtas * sizeof(PaDesc)) % 16 == 0, "the parts are 16-byte aligned");
   if (a.dtype == VVLI_BF16)
-    return a.head_dim == 64 ? queue_variant<__nv_bfloat16, 64>(device, p, a, ctas, s)
-                            : queue_variant<__nv_bfloat16, 128>(device, p, a, ctas, s);
-  return a.head_dim == 64 ? queue_variant<__half, 64>(device, p, a, ctas, s)
-                          : queue_variant<__half, 128>(device, p, a, ctas, s);
+    return a.head_dim == 64 ? queue_variant<__nv_bfloat16, 64>(p, a, ctas, s)
+                            : queue_variant<__nv_bfloat16, 128>(p, a, ctas, s);
+  return a.head_dim == 64 ? queue_variant<__half, 64>(p, a, ctas, s) : queue_variant<__half, 128>(p, a, ctas, s);
 }
 
 }  // namespace
@@ -577,22 +601,12 @@ cudaError_t pa_queue_combine(const PaParams& p, int ctas, cudaStream_t s) {
 
 cudaError_t pa_tensor_map(CUtensorMap* map, const void* cache, const vvli_paged_attn_args& a, uint32_t box_rows,
                           uint32_t box_slices) {
-  static std::once_flag once;
-  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult q;
-    void* f = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  });
-  if (!encode) return cudaErrorNotSupported;
   const cuuint64_t dims[4] = {64, a.kv_heads * a.page_size, a.head_dim / 64, a.pages};
   const cuuint64_t strides[3] = {a.head_dim * 2, 128, a.page_stride * 2};
   const cuuint32_t box[4] = {64, box_rows, box_slices, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r =
-      encode(map, a.dtype == VVLI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+      tensor_map_encode(map, a.dtype == VVLI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
              const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

@@ -431,11 +431,17 @@ VVLI_DEV void pa_add_not_finite(const PaParams& p, const PaSeg& s, int pos, int 
 }
 
 // ---------------------------------------------------------------- host
+template <class K>
+cudaError_t allow_smem(K kernel, size_t bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
 cudaError_t pa_tensor_map(CUtensorMap* map, const void* cache, const vvli_paged_attn_args& a, uint32_t box_rows,
                           uint32_t box_slices);
 // The tensor-core kernel (paged_attn_tc.cu) and, for either, the combine kernel (paged_attn.cu).
 template <class T, int D>
-cudaError_t pa_queue_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s);
+cudaError_t pa_set_up_tc();
+template <class T, int D>
+cudaError_t pa_queue_tc(const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s);
 template <class T, int D, int ROWS>
 cudaError_t pa_queue_combine(const PaParams& p, int ctas, cudaStream_t s);
 

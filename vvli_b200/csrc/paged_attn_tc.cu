@@ -29,7 +29,6 @@
 #include "tc_ptx.cuh"
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 namespace vvli {
@@ -722,16 +721,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <class T, int D, int FEAT>
-cudaError_t launch_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
-  static std::once_flag once[kOpMaxDevices];
-  static cudaError_t ready[kOpMaxDevices];
-  std::call_once(once[device], [&] {
-    ready[device] = cudaFuncSetAttribute(paged_tc_kernel<T, D, FEAT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         TcaLayout<D>::smem);
-  });
-  cudaError_t e = ready[device];
+cudaError_t launch_tc(const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
-  if (e == cudaSuccess) e = pa_tensor_map(&km, a.k_cache, a, static_cast<uint32_t>(a.page_size), 1);
+  cudaError_t e = pa_tensor_map(&km, a.k_cache, a, static_cast<uint32_t>(a.page_size), 1);
   if (e == cudaSuccess) e = pa_tensor_map(&vm, a.v_cache, a, static_cast<uint32_t>(a.page_size), 1);
   if (e != cudaSuccess) return e;
   paged_tc_kernel<T, D, FEAT><<<ctas, kTcThreads, TcaLayout<D>::smem, s>>>(p, km, vm);
@@ -742,17 +734,29 @@ cudaError_t launch_tc(int device, const PaParams& p, const vvli_paged_attn_args&
 }  // namespace
 
 template <class T, int D>
-cudaError_t pa_queue_tc(int device, const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
+cudaError_t pa_set_up_tc() {
+  cudaError_t e = allow_smem(paged_tc_kernel<T, D, 0>, TcaLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_tc_kernel<T, D, kPaCap>, TcaLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_tc_kernel<T, D, kPaAlibi>, TcaLayout<D>::smem);
+  if (e == cudaSuccess) e = allow_smem(paged_tc_kernel<T, D, kPaCap | kPaAlibi>, TcaLayout<D>::smem);
+  return e;
+}
+template <class T, int D>
+cudaError_t pa_queue_tc(const PaParams& p, const vvli_paged_attn_args& a, int ctas, cudaStream_t s) {
   switch (pa_features(p)) {
-    case 0: return launch_tc<T, D, 0>(device, p, a, ctas, s);
-    case kPaCap: return launch_tc<T, D, kPaCap>(device, p, a, ctas, s);
-    case kPaAlibi: return launch_tc<T, D, kPaAlibi>(device, p, a, ctas, s);
-    default: return launch_tc<T, D, kPaCap | kPaAlibi>(device, p, a, ctas, s);
+    case 0: return launch_tc<T, D, 0>(p, a, ctas, s);
+    case kPaCap: return launch_tc<T, D, kPaCap>(p, a, ctas, s);
+    case kPaAlibi: return launch_tc<T, D, kPaAlibi>(p, a, ctas, s);
+    default: return launch_tc<T, D, kPaCap | kPaAlibi>(p, a, ctas, s);
   }
 }
-template cudaError_t pa_queue_tc<__nv_bfloat16, 64>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
-template cudaError_t pa_queue_tc<__nv_bfloat16, 128>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
-template cudaError_t pa_queue_tc<__half, 64>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
-template cudaError_t pa_queue_tc<__half, 128>(int, const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
+template cudaError_t pa_set_up_tc<__nv_bfloat16, 64>();
+template cudaError_t pa_queue_tc<__nv_bfloat16, 64>(const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
+template cudaError_t pa_set_up_tc<__nv_bfloat16, 128>();
+template cudaError_t pa_queue_tc<__nv_bfloat16, 128>(const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
+template cudaError_t pa_set_up_tc<__half, 64>();
+template cudaError_t pa_queue_tc<__half, 64>(const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
+template cudaError_t pa_set_up_tc<__half, 128>();
+template cudaError_t pa_queue_tc<__half, 128>(const PaParams&, const vvli_paged_attn_args&, int, cudaStream_t);
 
 }  // namespace vvli

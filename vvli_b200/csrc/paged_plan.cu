@@ -13,7 +13,6 @@
 // more than the repeated scan.
 #include <algorithm>
 #include <climits>
-#include <mutex>
 
 #include "common.cuh"
 #include "op_common.cuh"
@@ -182,14 +181,13 @@ std::string check_plan(const vvli_paged_plan_args* a) {
 
 cudaError_t queue_plan(int device, const vvli_paged_plan_args& a, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(a.requests) * 4 * sizeof(int);  // <= 128 KB
-  static std::once_flag once[kOpMaxDevices];
-  static cudaError_t configured[kOpMaxDevices];
+  static SetupOnce setup[kOpMaxDevices];
   if (device < 0 || device >= kOpMaxDevices) return cudaErrorInvalidDevice;
-  std::call_once(once[device], [&] {
-    configured[device] = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              kPlanMaxRequests * 4 * sizeof(int));
+  const cudaError_t e = setup[device]([] {
+    return cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kPlanMaxRequests * 4 * sizeof(int));
   });
-  if (configured[device] != cudaSuccess) return configured[device];
+  if (e != cudaSuccess) return e;
   // One CTA while its threads take at most two rows each; the cluster beyond.
   const unsigned ctas = a.max_tokens <= 2 * kPlanThreads ? 1 : kPlanCluster;
   int shift = 4;
