@@ -593,10 +593,12 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * it picks the kernel, not the result (up to a rounding).  A call queues two
  * kernels.  Two calls that may run at the same time need a workspace each.
  * Limits: head_dim 64 or 128; q_heads a multiple of kv_heads, q_heads <= 512;
- * tokens * q_heads <= 2^31 - 1025; requests in [1, 65536]; window < 2^31; strides (elements) multiples of 8 and at least a
- * row; 16-bit pointers 16-byte aligned; workspace 256-byte aligned.  The first
- * int32 of the workspace is set to VVLI_ERR_TIMEOUT if a bounded wait gave up
- * (never cleared; zero it before the first call to read it). */
+ * tokens * q_heads <= 2^31 - 1025; requests in [1, 65536]; window < 2^31;
+ * scale * log2(e), softcap * log2(e) and scale / softcap finite in fp32;
+ * strides (elements) multiples of 8 and at least a row; 16-bit pointers
+ * 16-byte aligned; workspace 256-byte aligned.  The first int32 of the
+ * workspace is set to VVLI_ERR_TIMEOUT if a bounded wait gave up (never
+ * cleared; zero it before the first call to read it). */
 typedef struct vvli_paged_attn_args {
   uint64_t requests;
   uint64_t tokens;          /* rows of q and out */

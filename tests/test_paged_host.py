@@ -104,3 +104,12 @@ def test_wrappers_refuse_host_tensors():
         paged.qk_norm_rope_write(h, h, h, c, c, i)
     with pytest.raises(ValueError):
         speculative.verify_drafts(torch.zeros(4, 8), None, i, i, torch.zeros(4), torch.zeros(1))
+
+
+def test_attention_refuses_scores_out_of_range():
+    # scale / softcap past fp32 would make a score of 0 NaN, a cap or scale times log2(e) past it an infinity
+    lib = _abi.lib()
+    good = _abi.CPagedAttnArgs(4, 9, 14, 2, 64, 16, 10, 2 * 16 * 64, 5, 14 * 64, 14 * 64, 3, 0, 0, 0.125, 0.0, 0,
+                               *[PTR] * 10, lib.vvli_cuda_paged_attn_workspace_bytes(64))
+    for changes in ({"softcap": 1e-40}, {"softcap": 2e-38, "scale": -8.0}, {"softcap": 3e38}, {"scale": 3e38}, {"scale": -3e38}):
+        refused(lib.vvli_cuda_paged_attention, good, changes, "fp32")

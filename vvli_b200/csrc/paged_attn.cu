@@ -503,6 +503,8 @@ cudaError_t set_up_device(int device, int* sms) {
   return e;
 }
 
+constexpr double kLog2e = 1.44269504088896340736;
+
 std::string check_attn(const vvli_paged_attn_args* a) {
   if (!a) return "null arguments";
   if (a->requests < 1 || a->requests > 65536) return "requests must be in [1, 65536]";
@@ -525,6 +527,9 @@ std::string check_attn(const vvli_paged_attn_args* a) {
   if (a->dtype != VVLI_BF16 && a->dtype != VVLI_FP16) return "dtype must be VVLI_BF16 or VVLI_FP16";
   if (!std::isfinite(a->scale) || !(a->softcap >= 0.f) || std::isinf(a->softcap))
     return "scale must be finite, softcap finite and >= 0";
+  if (std::isinf(static_cast<float>(a->scale * kLog2e)) ||
+      (a->softcap > 0.f && (std::isinf(a->scale / a->softcap) || std::isinf(static_cast<float>(a->softcap * kLog2e)))))
+    return "scale, scale / softcap and softcap are too large or too small for fp32";
   const void* need[] = {a->q, a->k_cache, a->v_cache, a->out, a->block_table, a->cu_new, a->seq_len, a->workspace};
   for (int i = 0; i < 8; ++i) {
     if (!need[i] && !(a->tokens == 0 && (i == 0 || i == 3))) return "null pointer";
@@ -558,7 +563,6 @@ cudaError_t queue_attn(int device, const vvli_paged_attn_args& a, cudaStream_t s
   p.pages = static_cast<int>(a.pages), p.width = static_cast<int>(a.table_width);
   p.window = static_cast<int>(a.window);
   p.longest = static_cast<int>(std::min<uint64_t>(a.table_width * a.page_size, INT_MAX - 1024));
-  constexpr double kLog2e = 1.44269504088896340736;
   p.negate = a.scale < 0.f && !(a.softcap > 0.f) && !a.alibi;
   p.scale_log2 = static_cast<float>((p.negate ? -a.scale : a.scale) * kLog2e);
   if (a.softcap > 0.f) {
