@@ -219,3 +219,29 @@ def test_captures_of_variants_that_have_not_run():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     p = subprocess.run([sys.executable, "-c", CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
     assert p.returncode == 0 and p.stdout.endswith("captured\n"), p.stderr[-2000:]
+
+
+def test_a_step_without_requests():
+    import torch
+    from vvli_b200.paged import PagedAttention, plan_step, qk_norm_rope_write
+    from vvli_b200.speculative import verify_drafts
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    none, table = ints([]), ints([]).view(0, 4)
+    caches = [torch.zeros(3, HK, PAGE, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    attention = PagedAttention(HQ, HK, D, PAGE)
+    for rows in (0, 5):
+        for count, left in ((2, 2), (9, 3), (-1, 0)):
+            for inplace in (False, True):
+                free_count = ints([count])
+                step = plan_step(none, none, none, table, ints([2, 0, 1]), free_count, PAGE, rows, inplace=inplace)
+                assert [x.tolist() for x in step] == [[0], [], [0] * rows, [-1] * rows, [], [left], []]
+                assert free_count.tolist() == [left if inplace else count]
+        q, k = (torch.ones(rows, h, D, dtype=torch.bfloat16, device="cuda") for h in (HQ, HK))
+        q = qk_norm_rope_write(q, k, k, *caches, step.slots, step.positions)
+        assert not any(bool(c.any()) for c in caches)
+        out = torch.full((rows, HQ, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        assert attention(q, *caches, table, step.cu_new, step.seq_len, 0, out=out) is out and bool((out == 7).all())
+        assert attention(q, *caches, table, step.cu_new, step.seq_len, 0, lse=True)[1].shape == (rows, HQ)
+        accepted, tokens = verify_drafts(torch.ones(rows, 9, device="cuda"), None, step.positions, step.cu_new,
+                                         torch.ones(rows, device="cuda"), torch.ones(0, device="cuda"))
+        assert accepted.numel() == 0 and tokens.shape == (rows,)

@@ -121,6 +121,8 @@ def plan_step(context, new, owned, block_table, free_pages, free_count, page_siz
     if max_tokens < 0:
         raise ValueError("plan_step: max_tokens must be >= 0")
     sizes = (B + 1, B, max_tokens, max_tokens, B, 1, B)
+    if B == 0:
+        return _plan_of_nothing(owned, free_pages, free_count, dev, max_tokens, inplace, stream)
     buf = _empty(4 * B + 2 * max_tokens + 2, torch.int32, context.device, stream)
     cu = buf.data_ptr()
     seq = cu + 4 * (B + 1)
@@ -138,6 +140,19 @@ def plan_step(context, new, owned, block_table, free_pages, free_count, page_siz
     if inplace:
         out = (*out[:4], owned, free_count, out[6])
     return StepPlan(*out)
+
+
+def _plan_of_nothing(owned, free_pages, free_count, dev: int, max_tokens: int, inplace: bool, stream) -> StepPlan:
+    """The plan of a step without requests, which the library does not take."""
+    _ints("plan_step", "owned", owned, dev), _ints("plan_step", "free_pages", free_pages, dev)
+    _ints("plan_step", "free_count", free_count, dev, 1)
+    with torch.cuda.device(dev), torch.cuda.stream(stream):  # None: the current one
+        left = free_count[:1].clamp(0, free_pages.numel())
+        if inplace:
+            free_count[:1].copy_(left)
+        none, zeros = owned.new_empty(0), owned.new_zeros(1 + max_tokens)
+        return StepPlan(zeros[:1], none, zeros[1:], torch.full_like(zeros[1:], -1), owned if inplace else none,
+                        free_count if inplace else left, none)
 
 
 def qk_norm_rope_write(q, k, v, k_cache, v_cache, slots, positions=None, inv_freq=None, q_weight=None, k_weight=None,
@@ -265,7 +280,8 @@ class PagedAttention:
             self.window, self._type, self.scale, self.softcap, 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             out.data_ptr(), lp, self._alibi, _ints(who, "block_table", block_table, dev),
             _ints(who, "cu_new", cu_new, dev, B + 1), _ints(who, "seq_len", seq_len, dev), self._ws_at, self._ws_bytes)
-        check(_abi.lib().vvli_cuda_paged_attention(dev, a, _stream(dev, stream)))
+        if B:  # a step without requests writes nothing
+            check(_abi.lib().vvli_cuda_paged_attention(dev, a, _stream(dev, stream)))
         return out if lse is False else (out, lse)
 
     def status(self) -> int:

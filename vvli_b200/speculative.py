@@ -52,7 +52,7 @@ def verify_drafts(target, draft, tokens, cu_rows, u_accept, u_sample, stream=Non
     ua, us = _uniform("u_accept", u_accept, T, dev), _uniform("u_sample", u_sample, B, dev)
     tok, cu = _ints("verify_drafts", "tokens", tokens, dev, T), _ints("verify_drafts", "cu_rows", cu_rows, dev, B + 1)
     buf = _empty(B + T, torch.int32, target.device, stream)
-    if T == 0:  # no request has a row
+    if T == 0 or B == 0:  # no request has a row
         with torch.cuda.stream(stream):  # None: the current one
             buf.zero_()
     else:
