@@ -270,3 +270,17 @@ def test_qk_row_norm_in_place_over_many_heads(torch):
     inp = make_qk(torch, 11, 21, 96, 24, 128, 32, torch.bfloat16, "row", 64)
     for _ in range(3):
         check_qk(torch, inp, "row", False, inplace=True)
+
+
+@pytest.mark.parametrize("norm", ["none", "head", "row"])
+@pytest.mark.parametrize("T", [257, 1023, 1025, 2051])
+def test_qk_many_tokens(torch, norm, T):
+    # CTAs of one, two and eight tokens, the last of them with fewer
+    for hq, hk, d, pairs, interleaved in ((6, 2, 64, 32, True), (3, 3, 128, 32, False)):
+        inp = make_qk(torch, T, T, hq, hk, d, 16, torch.float16 if interleaved else torch.bfloat16, norm, pairs)
+        check_qk(torch, inp, norm, interleaved, inplace=T == 1025)
+
+
+def test_qk_row_norm_of_many_tokens_in_place_over_many_heads(torch):
+    inp = make_qk(torch, 12, 1037, 20, 10, 128, 32, torch.bfloat16, "row", 64)
+    check_qk(torch, inp, "row", False, inplace=True)

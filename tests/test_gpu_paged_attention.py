@@ -409,3 +409,35 @@ def test_values_that_are_not_finite_before_runs_of_narrow_items(torch, d, window
         assert torch.equal(out[odd & ~torch.isnan(want)], want[odd & ~torch.isnan(want)])
         assert float((out - want)[~odd].norm() / want[~odd].norm()) < 2 * torch.finfo(q.dtype).eps / 2  # as in check()
     assert att.status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("max_new", [1, 10**6])
+def test_many_short_requests(torch, d, max_new):
+    # more requests than threads of either kernel: the shares are worked out in several rounds
+    r = random.Random(d)
+    lens = [(n + r.randint(0, 90), n) for n in (r.randint(0, 6) for _ in range(900))]
+    check(torch, make(torch, 13, lens, 4, 2, d, 16, torch.bfloat16), 16, max_new=max_new)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "float16"), (128, "bfloat16")])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (60, 0.0), (60, 20.0)])
+@pytest.mark.parametrize("max_new", [1, 10**6])
+def test_keys_that_are_not_finite(torch, d, dtype, window, softcap, max_new):
+    # A NaN key makes the rows that see it NaN, an infinite one those that it scores +inf (a score of -inf has no
+    # weight, a cap makes either finite); rows that do not, earlier in the block or past the window, have nothing of it.
+    from vvli_b200.paged import PagedAttention
+    lens = [(90, 5), (300, 200), (64, 64), (700, 3), (500, 40), (130, 1)]
+    q, k, v, table, cu, seq = make(torch, 27, lens, 8, 2, d, 16, getattr(torch, dtype), poison=False)
+    r = random.Random(3)
+    for b, (e, n) in enumerate(lens):
+        for h, value in enumerate((math.nan, math.inf)):
+            key = e - 1 - r.randrange(min(e, n + 70 if window else n))
+            k[table[b][key // 16], h, key % 16, r.randrange(d)] = value
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    att = PagedAttention(8, 2, d, 16, dtype=q.dtype, window=window, softcap=softcap)
+    out = att(q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), max_new).cpu().double()
+    want, _ = ref.attention(q, k, v, table, cu, seq, d**-0.5, window, softcap)
+    nan = torch.isnan(want)
+    assert int(nan.sum()) > 100 and int((~nan).sum()) > 100 and torch.equal(torch.isnan(out), nan)
+    assert float((out - want)[~nan].norm() / want[~nan].norm()) < 2 * torch.finfo(q.dtype).eps / 2  # as in check()

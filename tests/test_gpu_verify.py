@@ -136,3 +136,31 @@ def test_errors(torch):
             bad()
     acc, out = verify_drafts(t[:0], None, i[:0], i, u[:0], u[:3])
     assert acc.tolist() == [0, 0, 0] and out.numel() == 0
+
+
+@pytest.mark.parametrize("V", [196608, 196609, 256000, 262144])
+@pytest.mark.parametrize("one_hot", [False, True])
+def test_large_vocabularies(torch, V, one_hot):
+    # up to and past the slice whose runs a thread holds in registers
+    target, draft, tokens, cu, ua, us = make(torch, V, [1, 3, 2, 4], V)
+    check(torch, target, None if one_hot else draft, tokens, cu, ua, us)
+    us[:] = torch.tensor([0.0, 1.0 - 2.0**-24, 1.0, 0.999])
+    check(torch, target, None if one_hot else draft, tokens, cu, ua + 1e6, us)
+
+
+def test_repeats(torch):
+    lengths = [1 + i % 6 for i in range(100)]
+    args = make(torch, 6, lengths, 32003)
+    first = run(torch, *args)
+    assert all(run(torch, *args) == first for _ in range(3))
+
+
+def test_rows_behind_the_last_request_are_left(torch):
+    from vvli_b200 import _abi
+    target, draft, tokens, cu, ua, us = make(torch, 14, [3, 0, 4, 5], 500)
+    dev = [x.cuda() for x in (target, draft, tokens, torch.tensor(cu[:-1], dtype=torch.int32), ua, us)]
+    acc, out = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (4, 12))
+    a = _abi.pack_verify(3, 12, 500, 500, 500, *[x.data_ptr() for x in dev], acc.data_ptr(), out.data_ptr())
+    assert _abi.lib().vvli_cuda_verify_drafts(0, a, torch.cuda.current_stream().cuda_stream) == 0
+    want = ref.verify(target, draft, tokens, cu[:-1], ua, us)
+    assert acc.tolist() == want[0] + [77] and out.tolist() == [77 if w is None else w for w in want[1]]
