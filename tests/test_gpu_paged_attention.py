@@ -441,3 +441,35 @@ def test_keys_that_are_not_finite(torch, d, dtype, window, softcap, max_new):
     nan = torch.isnan(want)
     assert int(nan.sum()) > 100 and int((~nan).sum()) > 100 and torch.equal(torch.isnan(out), nan)
     assert float((out - want)[~nan].norm() / want[~nan].norm()) < 2 * torch.finfo(q.dtype).eps / 2  # as in check()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_workspace_on_other_streams(torch, new):
+    # The workspace's memory may be on its way from another use, and back to one: neither shows, whatever stream a
+    # call is on, and although the object goes away while its call still runs.
+    from vvli_b200.paged import PagedAttention
+    q, k, v, table, cu, seq = make(torch, 33, [(3000, new), (40 + new, new)], 8, 2, 128, 64, torch.bfloat16, poison=False)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = (q.cuda(), k.cuda(), v.cuda(), ints(table), ints(cu), ints(seq), new)
+    want = PagedAttention(8, 2, 128, 64)(*args).cpu()
+    size = PagedAttention(8, 2, 128, 64)._ws.numel()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for given in (True, False):
+        before = torch.empty(size, dtype=torch.uint8, device="cuda")
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        before.fill_(255)
+        at = before.data_ptr()
+        del before
+        att = PagedAttention(8, 2, 128, 64)
+        assert att._ws.data_ptr() == at  # the same memory, the point of the test
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            out = att(*args, stream=side if given else None)
+        del att
+        after = torch.empty(size, dtype=torch.uint8, device="cuda")
+        assert after.data_ptr() != at
+        after.fill_(255)
+        side.synchronize()
+        assert torch.equal(out.cpu(), want)
+        torch.cuda.synchronize()

@@ -219,6 +219,8 @@ class PagedAttention:
     position - query position) when alibi (float32 [q_heads]) is given.  The
     workspace (its size depends on head_dim alone) is allocated here: calls of
     one object, and graphs captured from them, must not run at the same time.
+    Calls may be on any streams, which have to outlive the object; a graph of
+    its calls must not be replayed once it is gone.
     """
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, page_size: int, dtype=torch.bfloat16, scale=None,
@@ -245,9 +247,13 @@ class PagedAttention:
         if self.window < 0:
             raise ValueError("PagedAttention: window must be >= 0")
         self._type, self._alibi = _DTYPES[dtype], 0 if alibi is None else alibi.data_ptr()
-        self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        self._ws[:4].zero_()
-        self._ws_at, self._ws_bytes = self._ws.data_ptr(), need
+        with torch.cuda.device(self.device):
+            self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            self._ws[:4].zero_()
+            home = torch.cuda.current_stream()
+            if not torch.cuda.is_current_stream_capturing():
+                home.synchronize()  # calls may be on any stream: what the memory was used for before is over
+        self._ws_at, self._ws_bytes, self._streams = self._ws.data_ptr(), need, {home.cuda_stream}
 
     def __call__(self, q, k_cache, v_cache, block_table, cu_new, seq_len, max_new: int, out=None, lse=False, stream=None):
         """q: [rows][q_heads][head_dim]; block_table: int32 [requests][width]; cu_new: int32 [requests + 1] and seq_len:
@@ -280,8 +286,12 @@ class PagedAttention:
             self.window, self._type, self.scale, self.softcap, 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             out.data_ptr(), lp, self._alibi, _ints(who, "block_table", block_table, dev),
             _ints(who, "cu_new", cu_new, dev, B + 1), _ints(who, "seq_len", seq_len, dev), self._ws_at, self._ws_bytes)
+        s = _stream(dev, stream)
+        if s not in self._streams:  # the workspace goes back to the allocator when that stream is done with it, too
+            self._ws.record_stream(torch.cuda.current_stream(dev) if stream is None else stream)
+            self._streams.add(s)
         if B:  # a step without requests writes nothing
-            check(_abi.lib().vvli_cuda_paged_attention(dev, a, _stream(dev, stream)))
+            check(_abi.lib().vvli_cuda_paged_attention(dev, a, s))
         return out if lse is False else (out, lse)
 
     def status(self) -> int:
