@@ -534,7 +534,7 @@ int vvli_cuda_paged_plan(int device, const vvli_paged_plan_args* args, void* str
  *   q goes to q_out (which may be q), k and v (unnormed, unturned) to the
  *       cache position slots[t] = page * page_size + offset.  A slot outside
  *       the cache, -1 among them, writes no k and v.  Two rows with the same
- *       slot leave either's values.
+ *       slot leave a mixture of their values.
  * Arithmetic in fp32, rounded once to the 16-bit type.
  * Limits: head_dim a multiple of 16 in [16, 256], rotary_pairs a multiple of 8
  * with 2 * rotary_pairs <= head_dim, q_heads and kv_heads in [1, 512], tokens <
@@ -583,7 +583,8 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * (p < 0) gets out 0 and lse -inf; rows from cu_new[requests] on are left as
  * they were.  What a row does not see does not reach it, whatever its bits
  * (infinities and NaN among them), and what the cache holds past a request's
- * seq_len is never used.  Keys whose table entry is outside [0, pages) count as
+ * seq_len is never used.  A score of +inf or NaN that a row sees makes it, and
+ * its lse, NaN.  Keys whose table entry is outside [0, pages) count as
  * zero keys and values.  cu_new must not decrease and is cut at `tokens`,
  * seq_len at table_width * page_size.  Products of 16-bit values summed in fp32; the
  * probabilities enter the second product rounded to the 16-bit type (fp16: half a
