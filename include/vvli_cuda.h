@@ -588,7 +588,7 @@ int vvli_cuda_qk_rope_write(int device, const vvli_qk_rope_args* args, void* str
  * zero keys and values.  cu_new must not decrease and is cut at `tokens`,
  * seq_len at table_width * page_size.  Products of 16-bit values summed in fp32; the
  * probabilities enter the second product rounded to the 16-bit type (fp16: half a
- * step of those down to 2^-25 of the row's largest, and none below 2^-36 of it);
+ * step of those down to 2^-23 of the row's largest, and none below 2^-34 of it);
  * results do not depend on timing.
  * `max_new` is the longest request's new tokens as far as the caller knows:
  * it picks the kernel, not the result (up to a rounding).  A call queues two

@@ -374,9 +374,11 @@ def test_dominant_keys_of_no_value_leave_the_others(torch, dtype, gap, new):
         ints([30000] * B), new, lse=True)
     want, wlse = ref.attention(q, k, v, table, [0, new], [30000], 64**-0.5)
     # Values of one sign, so the errors of the terms bound that of the sum, relative to it: the output's
-    # rounding, that of a probability (half a step; in fp16 e^-18.3 is 2^-26.4, held as 2^-15.4 at least, where
-    # a half's spacing is 2^-24: 2^-9.6), 2^-11 for score and exponential as in check(), and 2^-13 for fp32
-    # sums over 30,000 keys, 16 at a time.
+    # rounding, that of a probability (half a step; in fp16 e^-18.3 is 2^-26.4, held as 2^-17.4 at least, where a
+    # half's spacing is 2^-24, so that a term is off by up to 2^-7.6, but in either direction: spread over some 46
+    # spacings, 29,880 of them together by 2^-7.6 / sqrt(3 * 29,880) = 2^-15.8, six times which is well below the
+    # 2^-9.6 allowed), 2^-11 for score and exponential as in check(), and 2^-13 for fp32 sums over 30,000 keys,
+    # 16 at a time.
     half = torch.finfo(dtype).eps / 2
     off = float(((out.cpu().double().view(B, new, 4, 64) - want).abs() / want).max())
     assert off < half + max(half, 2.0**-9.6) + 2.0**-11 + 2.0**-13

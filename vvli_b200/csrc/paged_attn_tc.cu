@@ -12,7 +12,7 @@
 //     to the 16-bit type, goes back over the same columns, from where it is the
 //     A operand of O_t += P_t V; O_t stays in TMEM.  A row's O is rescaled only
 //     when its maximum rises by more than 2^8 (P then stays below 2^8; in fp16
-//     2^4 and 2^15), which after a row's first tiles is rare.
+//     2^6 and 2^15), which after a row's first tiles is rare.
 //   * K and V tiles come by TMA, a box per page and 64-element slice, into a
 //     128 KB ring in the 128-byte-swizzled layout; V is read as it lies (keys by
 //     rows) through an MN-major descriptor, so nothing is transposed.
@@ -42,9 +42,11 @@ constexpr int kTcOdd = 8;        // segments of a row tile whose key tiles with 
 // An item's start and end count as this many tiles (4,096 new tokens at head_dim 64:
 // 172 us with none, 155 with 1, 134 with 2, 127 with 3; others alike from 2 on).
 constexpr int kTcExtra = 3;
-// A row maximum's rise (log2) that rescales its output: 2^8, in fp16 2^4 above a reference 2^11 below it (paged_attn.cuh).
+// A row maximum's rise (log2) that rescales its output: 2^8, in fp16 2^6 above a
+// maximum 2^9 above the reference (paged_attn.cuh).  4,096 rows over 8,192 keys in
+// fp16: 389 us with 2^8 and 2^7, 386 so, 391 with 2^5 and 2^10, 411 with 2^4 and 2^11.
 template <class T>
-constexpr float kTcRise = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+constexpr float kTcRise = std::is_same<T, __half>::value ? 6.0f : 8.0f;
 
 template <int D>
 struct TcaLayout {
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int pos = live ? sg.r.pos0 + tok : -1;
       const int first_pos = sg.r.pos0 + pa_div_g(p, sg.blk * kTcRows + row0);  // of this tile's first row
       const int last_pos = sg.it.hi - 1;
-      constexpr float kLift = pa_lift<T>(11.f);
+      constexpr float kLift = pa_lift<T>(9.f);
       float m = -INFINITY, l = 0.f;  // the row's reference, and its sum relative to it
       const float slope = (FEAT & kPaAlibi) && p.alibi && live ? p.alibi[head] * 1.44269504088896340736f : 0.f;
       if (nt > 0 && !dead) {
