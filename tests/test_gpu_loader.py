@@ -249,3 +249,42 @@ def test_gguf_errors(oracle, vv, tmp_path):
     p.write_bytes(good)
     gpu.load_gguf(str(p))
     assert gpu.forward_token(1, 0).shape == (cfg.vocab_size,)
+
+
+JUST_WRITTEN = """
+import sys
+import numpy as np
+sys.path.insert(0, "tests")
+import vvli_b200
+from test_gpu_loader import C, bf16_tensors, logits_of, write_file, write_model
+from test_gpu_quant import G, gguf_llama, write_quantized_model
+import oracle
+cfg = gguf_llama(1024, 16, 4, 2816, 2, 16384)
+path = sys.argv[1]
+for seed in range(4):
+    blob = oracle.synthetic_blob(cfg, seed=seed)
+    want = vvli_b200.Runner(cfg, max_seq=8)
+    want.load_weights(blob)
+    got = vvli_b200.Runner(cfg, max_seq=8)
+    write_file(path, bf16_tensors(cfg, blob))
+    got.load_safetensors(path)
+    assert np.array_equal(logits_of(got, [1, 2]), logits_of(want, [1, 2]))
+    write_model(path, cfg, blob, G.F32)
+    got.load_gguf(path)
+    assert np.array_equal(logits_of(got, [1, 2]), logits_of(want, [1, 2]))
+    write_quantized_model(path, cfg, blob, G.Q8_0)
+    got.load_gguf(path)
+    assert got.query("quantized") == 1
+print("loaded")
+"""
+
+
+def test_files_that_were_just_written_load(tmp_path):
+    # Pages that are still to be written back: page-locking them once kept a load in the kernel without end.  A process
+    # of its own, so that a time limit can end it.
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([root, os.path.join(root, "oracle"), os.environ.get("PYTHONPATH", "")]))
+    p = subprocess.run([sys.executable, "-c", JUST_WRITTEN, str(tmp_path / "model")], cwd=root, env=env, capture_output=True,
+                       text=True, timeout=180)
+    assert p.returncode == 0 and p.stdout.endswith("loaded\n"), p.stderr[-2000:]

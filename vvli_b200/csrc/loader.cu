@@ -11,9 +11,12 @@
 //   * BF16 rows are copied with one strided copy per piece; F32 rows are copied
 //     to a device staging buffer and rounded with the reference's f32ToBf16
 //     (round to nearest even, no NaN special case) by a kernel;
-//   * the mapping is page-locked read-only (cudaHostRegister) when the system
-//     allows it, so the copies are DMA from the page cache; otherwise they go
-//     through the driver's pageable path.
+//   * the mapping stays pageable, and the copies go through the driver's staging
+//     buffers.  Page-locking it (cudaHostRegister) would make them DMA from the
+//     page cache, but the kernel has to move page-cache pages before it pins them
+//     for long, and tries again without end while it cannot: loading files that
+//     had just been written, the call was seen not to come back for 25 minutes,
+//     all of them spent in the kernel with the GPU idle.
 //
 // loadGgufIntoOwnedModel (src/llm.zig:1008-1065) does the same for a GGUF
 // file (src/gguf.zig): the binary header and tensor table are parsed here,
@@ -227,9 +230,7 @@ struct Mapping {
   int fd = -1;
   void* base = MAP_FAILED;
   size_t size = 0;
-  bool registered = false;
   ~Mapping() {
-    if (registered) cudaHostUnregister(base);
     if (base != MAP_FAILED) munmap(base, size);
     if (fd >= 0) close(fd);
   }
@@ -254,12 +255,6 @@ struct Mapping {
     return VVLI_OK;
   }
   const uint8_t* bytes() const { return base == MAP_FAILED ? nullptr : static_cast<const uint8_t*>(base); }
-  // DMA straight from the page cache when the mapping can be page-locked.
-  void lock() {
-    if (base == MAP_FAILED) return;
-    registered = cudaHostRegister(base, size, cudaHostRegisterReadOnly) == cudaSuccess;
-    if (!registered) cudaGetLastError();
-  }
 };
 
 enum SrcType { kSrcBF16, kSrcF32, kSrcF16, kSrcQ8_0, kSrcQ4_0 };
@@ -599,7 +594,6 @@ int upload_safetensors(const char* path, const std::vector<LoadPiece>& pieces, i
   }
   const uint8_t* data = bytes + 8 + header_len;
   const size_t data_len = m.size - 8 - header_len;
-  m.lock();
   // copyTensorIntoWeight (src/llm.zig:1149-1183): name, dtype BF16 or F32,
   // element count and byte range.
   auto lookup = [&](uint64_t id, uint64_t expect, SrcTensor* t, std::string* err) -> int {
@@ -646,7 +640,6 @@ int upload_gguf(const char* path, const std::vector<LoadPiece>& pieces, int laye
   std::map<std::string, GgufTensor> tensors;
   uint64_t data_start = 0;
   if ((st = parse_gguf(m.bytes(), m.size, &tensors, &data_start, why)) != VVLI_OK) return st;
-  m.lock();
   // copyGgufTensorIntoWeight (src/llm.zig:1081-1138): name, native float
   // type (F32, F16, BF16), element count, byte range.
   auto lookup = [&](uint64_t id, uint64_t expect, SrcTensor* t, std::string* err) -> int {
