@@ -361,12 +361,14 @@ VVLI_DEV float pa_capped(float s, const PaParams& p) {
 // requests x 5 rows (0.5B heads), 75 -> 97 us for 16 mixed requests with a cap, and
 // 285.5 -> 290.5 us in the streaming kernel at 16 x 24,000 to 32,767 keys, where
 // infinite values times what is left (0 or less) would have to be kept out as
-// well.  Scores, maxima, sums and parts are fp32.  bf16 has fp32's exponents; fp16 loses bits below 2^-14 and holds nothing
-// below 2^-25, so there the reference is LIFT below the row's maximum: with it at
-// the maximum, 30,000 keys 18 (natural units) below a few dominant ones vanished from the
-// output while the sum counted them.  The sums and the log-sum-exp are relative
-// to the same reference.  LIFT bits and what a maximum may rise above its
-// reference stay below 2^16, fp16's end; from 2^22 on the difference would round.
+// well.  Scores, maxima, sums and parts are fp32.
+// bf16 has fp32's exponents; fp16 loses bits below 2^-14 and holds nothing below
+// 2^-25, so there the reference is `fp16_bits` (log2) below the row's maximum: with
+// it at the maximum, 30,000 keys 18 (natural units) below a few dominant ones
+// vanished from the output while the sum counted them.  The sums and the
+// log-sum-exp are relative to the same reference.  2^fp16_bits times what a
+// maximum may rise before the reference follows stays below 2^16, fp16's end;
+// for maxima from 2^22 on the difference would round, and the reference is the maximum.
 template <class T>
 constexpr float pa_lift(float fp16_bits) {
   return std::is_same<T, __half>::value ? fp16_bits : 0.f;
